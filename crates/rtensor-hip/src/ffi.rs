@@ -35,6 +35,8 @@ pub const RT_F32: c_int = 0;
 pub const RT_BF16: c_int = 1;
 pub const RT_F16: c_int = 2;
 pub const RT_U32: c_int = 3;
+pub const RT_MXFP4: c_int = 4;
+pub const RT_MXFP8: c_int = 5;
 
 // rt_layout
 pub const RT_NN: c_int = 0;
@@ -109,7 +111,11 @@ extern "C" {
     pub fn rt_free(ctx: *mut RtCtx, buf: *mut RtBuf) -> c_int;
     pub fn rt_buf_info(buf: *const RtBuf, dtype: *mut c_int, shape: *mut usize, rank: *mut c_int) -> c_int;
     pub fn rt_upload_labels(ctx: *mut RtCtx, labels: *const u64, n: usize, out: *mut *mut RtBuf) -> c_int;
+    pub fn rt_wrap(ctx: *mut RtCtx, dtype: c_int, shape: *const usize, rank: c_int, ptr: *mut c_void,
+                   out: *mut *mut RtBuf) -> c_int;
+    pub fn rt_tensor_bytes(dtype: c_int, shape: *const usize, rank: c_int) -> usize;
     pub fn rt_convert(ctx: *mut RtCtx, src: *const RtBuf, dst: *mut RtBuf) -> c_int;
+    pub fn rt_convert_t(ctx: *mut RtCtx, src: *const RtBuf, dst: *mut RtBuf) -> c_int;
 
     // Kernels (op_matmul*, ops_split_k, ops_colsum, op_softmax_xent, op_adam).
     pub fn rt_gemm(ctx: *mut RtCtx, layout: c_int, a: *const RtBuf, b: *const RtBuf, c: *mut RtBuf, epi: c_int,

@@ -52,7 +52,19 @@ typedef enum {
   RT_ERR_OVERFLOW = 8     /* non-finite gradient under loss scaling          */
 } rt_status;
 
-typedef enum { RT_F32 = 0, RT_BF16 = 1, RT_F16 = 2, RT_U32 = 3 } rt_dtype;
+/* RT_MXFP4 and RT_MXFP8 are microscaled floating point: tensors of rank 2 whose
+ * rows are cut into blocks of 32 columns with one scale 2^e each.  RT_MXFP4 holds
+ * e2m1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), RT_MXFP8 e4m3
+ * ones (up to 448, no infinities).  A buffer of R rows and C columns, with
+ * P = C rounded up to a multiple of 128, holds
+ *   - the codes: R rows of P/2 (RT_MXFP4: the even column in the low half of its
+ *     byte) or P bytes, zero past column C;
+ *   - from the next multiple of 256 bytes on, the scale bytes (e + 127; 255 makes
+ *     the block NaN), in the order in which the matrix units take them: for each
+ *     128 columns, for each 64 rows (the last may be short), 256 bytes of which
+ *     byte 4·(16·g + r) + t is that of row 16·t + r and columns 32·g .. 32·g+31.
+ * rt_tensor_bytes gives the size; transfers move the bytes as they are. */
+typedef enum { RT_F32 = 0, RT_BF16 = 1, RT_F16 = 2, RT_U32 = 3, RT_MXFP4 = 4, RT_MXFP8 = 5 } rt_dtype;
 
 /* C = A·B, Aᵀ·B (A stored [K, M]) or A·Bᵀ (B stored [N, K]). */
 typedef enum { RT_NN = 0, RT_TN = 1, RT_NT = 2 } rt_layout;
@@ -95,9 +107,35 @@ int rt_free(rt_ctx* ctx, rt_buf* buf);
 int rt_buf_info(const rt_buf* buf, rt_dtype* dtype, size_t* shape, int* rank);
 /* upload_labels (mod.rs:1672-1675): usize labels -> u32 device buffer. */
 int rt_upload_labels(rt_ctx* ctx, const uint64_t* labels, size_t n, rt_buf** out);
+/* A buffer over device memory that the caller owns: a tensor of another library,
+ * a slice of the caller's arena.  ptr is on the context's device, aligned to the
+ * element (RT_MXFP*: to 16 bytes), with rt_tensor_bytes bytes inside one
+ * allocation.  rt_free gives up the handle only.  The memory outlives the handle
+ * and the work enqueued on it, and the caller orders other streams' use of it
+ * against the context's (rt_sync, or a device synchronisation). */
+int rt_wrap(rt_ctx* ctx, rt_dtype dtype, const size_t* shape, int rank, void* ptr, rt_buf** out);
+/* Bytes of a tensor (what rt_upload and rt_download move); 0 for a bad dtype or
+ * shape, and for a tensor without elements. */
+size_t rt_tensor_bytes(rt_dtype dtype, const size_t* shape, int rank);
 /* f32 -> bf16/f16 with round-to-nearest-even, or half -> f32 (same shape):
- * upload_f16 / op_empacota_f16 (mod.rs:1151-1185, EMPACOTA mista.rs:326-341). */
+ * upload_f16 / op_empacota_f16 (mod.rs:1151-1185, EMPACOTA mista.rs:326-341).
+ *
+ * Between f32/bf16/f16 and RT_MXFP4/RT_MXFP8 (rank 2, same shape; no counterpart
+ * in the reference): a block's scale is the least power of two, from 2^-127 on,
+ * at which its largest finite magnitude does not pass 6 (RT_MXFP4) or 448
+ * (RT_MXFP8), and its elements are rounded to nearest, ties to even: each is
+ * within half a step of its value, and none saturates.  An infinity or NaN makes
+ * its RT_MXFP4 block NaN; in RT_MXFP8 it alone becomes NaN.  In RT_MXFP8 a value
+ * that rounds to zero is stored as code 0x80 if it was positive and 0 if not, so
+ * that 1[x > 0] of finite values can be read from the codes exactly.  Back, each
+ * code's value is rounded once to dst's type (f32 holds all but RT_MXFP4's 2^128,
+ * which a magnitude from 3.5·2^126 on rounds to and which becomes an infinity;
+ * bf16 also lacks those below 2^-133). */
 int rt_convert(rt_ctx* ctx, const rt_buf* src, rt_buf* dst);
+/* rt_convert of the transpose: src f32/bf16/f16 [R, C] into dst RT_MXFP4/RT_MXFP8
+ * [C, R], blocks along R: how a weight [in, out] is laid out for rt_gemm's RT_NT
+ * product.  No counterpart in the reference. */
+int rt_convert_t(rt_ctx* ctx, const rt_buf* src, rt_buf* dst);
 
 /* ------------------------------------------------------------- ops */
 
@@ -118,7 +156,7 @@ int rt_gemm(rt_ctx* ctx, rt_layout layout, const rt_buf* a, const rt_buf* b, rt_
  * mod.rs:1432-1467): dW = Xᵀ·δ [K, N], db = 1ᵀ·δ [N] (NULL to skip) and
  * dX = δ·Wᵀ [M, K] (NULL to skip), with X [M, K], δ [M, N], W [K, N].  f32
  * shapes the paired kernel takes run as ONE launch; anything else is the two
- * rt_gemm calls. */
+ * rt_gemm calls.  X may be RT_MXFP8: the input as it was saved in 8 bits. */
 int rt_linear_backward(rt_ctx* ctx, const rt_buf* x, const rt_buf* delta, const rt_buf* w, rt_buf* dx, rt_buf* dw,
                        rt_buf* db);
 
@@ -151,7 +189,8 @@ int rt_colsum(rt_ctx* ctx, const rt_buf* src, rt_buf* dst);
 int rt_bias_add(rt_ctx* ctx, rt_buf* z, const rt_buf* b);
 /* op_relu (mod.rs:765-775): Y = max(X, 0). */
 int rt_relu(rt_ctx* ctx, const rt_buf* x, rt_buf* y);
-/* op_relu_bwd (mod.rs:778-788): δ ← δ ⊙ 1[A > 0] in place. */
+/* op_relu_bwd (mod.rs:778-788): δ ← δ ⊙ 1[A > 0] in place.  A may be RT_MXFP8
+ * (as a mask of rt_gemm). */
 int rt_relu_bwd(rt_ctx* ctx, const rt_buf* a, rt_buf* delta);
 /* op_softmax_xent (mod.rs:791-808): per row loss -ln(max(p_y, 1e-12)) into
  * loss_rows[B] and δ = (softmax(z) - onehot(y)) * (scale / B).  Labels >= C
@@ -298,7 +337,8 @@ typedef enum {
 int rt_map(rt_ctx* ctx, rt_unary_op op, float k, const rt_buf* x, rt_buf* y);
 /* The VJP closure of op (ops.rs:132-227): dx from the upstream g, the op's
  * input x and its output y.  x is needed by SQUARE, LN, RELU, LEAKY_RELU;
- * y by SQRT, EXP, SIGMOID, TANH; either may be NULL when unused. */
+ * y by SQRT, EXP, SIGMOID, TANH; either may be NULL when unused.  For RT_U_RELU
+ * x may be RT_MXFP8 (as a mask of rt_gemm), g and dx then of its shape. */
 int rt_map_vjp(rt_ctx* ctx, rt_unary_op op, float k, const rt_buf* g, const rt_buf* x, const rt_buf* y,
                rt_buf* dx);
 /* Tensor::zip (tensor.rs:183-246) with numpy broadcasting

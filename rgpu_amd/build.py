@@ -31,6 +31,9 @@ SOURCES = {
     "optim.hip": ["-ffp-contract=off"],
     "tensor_ops.hip": ["-ffp-contract=off"],
     "noalloc.hip": [],
+    "mx.hip": [],
+    "mx_gemm.hip": [],
+    "mx_backward.hip": [],
 }
 
 COMMON = [

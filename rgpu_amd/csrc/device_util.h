@@ -75,6 +75,14 @@ __device__ inline void dma16_asm(__amdgpu_buffer_rsrc_t rsrc, void* lds, int vof
                "s"(so)
                : "m0");
 }
+
+// The same with 4 bytes a lane: into LDS at lds + 4 * lane.
+__device__ inline void dma4_asm(__amdgpu_buffer_rsrc_t rsrc, void* lds, int voff, int soff) {
+  const int so = __builtin_amdgcn_readfirstlane(soff);
+  const unsigned dst = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) void*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(dst), "v"(voff), "s"(rsrc), "s"(so)
+               : "m0");
+}
 #pragma clang diagnostic pop
 
 }  // namespace rt_dev

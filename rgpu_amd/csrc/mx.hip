@@ -1,0 +1,377 @@
+// Microscaled tensors: conversion to and from f32/bf16/f16, and the ReLU mask
+// of an 8-bit saved activation.  The layout is rtensor_hip.h's; all HBM-bound.
+//
+// Quantisation of a block of 32: with m·2^E, 1 <= m < 2, its largest finite
+// magnitude, the least e with m·2^E <= MAX·2^e is E - T, plus one if m is
+// above MAX's mantissa (MAX = 6 = 1.5·2^2 or 448 = 1.75·2^8), but not below
+// -127; so the scale byte is the exponent field of that magnitude less T (plus
+// one), and no element can round past MAX.  x·2^-e is exact, so the one
+// rounding is the hardware's conversion (round to nearest even).
+
+#include <type_traits>
+
+#include "mx_device.h"
+#include "rt_internal.h"
+
+namespace {
+
+using rt_mx::u2;
+using rt_mx::u4;
+
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef short s2 __attribute__((ext_vector_type(2)));
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+  static __device__ inline float get(float v) { return v; }
+  static __device__ inline float put(float v) { return v; }
+};
+struct bf16_bits {
+  unsigned short u;
+};
+template <>
+struct Elem<bf16_bits> {
+  static __device__ inline float get(bf16_bits v) { return __uint_as_float((unsigned)v.u << 16); }
+  static __device__ inline bf16_bits put(float v) { return bf16_bits{rt_mx::f32_to_bf16(v)}; }
+};
+template <>
+struct Elem<_Float16> {
+  static __device__ inline float get(_Float16 v) { return (float)v; }
+  static __device__ inline _Float16 put(float v) { return (_Float16)v; }
+};
+
+// The scale byte for the largest magnitude's bits of a block.
+template <bool FP4>
+__device__ inline unsigned scale_byte(unsigned amax) {
+  constexpr unsigned top = FP4 ? 2 : 8, mant = FP4 ? 0x400000 : 0x600000;
+  const unsigned e = (amax >> 23) + ((amax & 0x7fffffu) > mant ? 1u : 0u);
+  return e > top ? e - top : 0u;
+}
+
+// What a value's magnitude counts for in the block's maximum: RT_MXFP8 leaves
+// out infinities and NaN (they become NaN codes beside whatever scale the
+// others want), RT_MXFP4 keeps them (its block becomes NaN).
+template <bool FP4>
+__device__ inline unsigned magnitude(float v) {
+  const unsigned m = __float_as_uint(v) & 0x7fffffffu;
+  return FP4 || m < 0x7f800000u ? m : 0u;
+}
+
+// Four values as four 4-bit (low 16 bits of the result) or 8-bit codes.
+template <bool FP4>
+__device__ inline unsigned encode4(const float* v, float scale) {
+  if constexpr (FP4) {
+    unsigned w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], scale, 0);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1) & 0xffffu;
+  } else {
+    s2 h = {0, 0};
+    h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, v[0], v[1], scale, false);
+    h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, v[2], v[3], scale, true);
+    const unsigned w = __builtin_bit_cast(unsigned, h);
+    // Zero codes take 0x80 where the value was positive, 0 where it was not.
+    const unsigned nonzero = ((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) & 0x80808080u;
+    unsigned pos = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pos |= v[i] > 0.0f ? 0x80u << (8 * i) : 0u;
+    return (w & (0x7f7f7f7fu | nonzero)) | (pos & ~nonzero);
+  }
+}
+
+// Stores the scale bytes of a 64-row group of one step, gathered in LDS in the
+// order of the layout.  Rows past the last one hold zeros.
+__device__ inline void store_scales(const unsigned* sc, unsigned char* scales, long long step, long long groups,
+                                    long long group) {
+  if (threadIdx.x < 64)
+    reinterpret_cast<unsigned*>(scales)[(step * groups + group) * 64 + threadIdx.x] = sc[threadIdx.x];
+}
+
+// A block of threads takes 64 rows of one step (128 columns): lanes hold V
+// consecutive values (16 bytes), so 32 / V lanes share a block and find its
+// maximum by exchange.
+template <typename T, bool FP4>
+__global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ src, long long rows, long long cols,
+                                                       unsigned char* __restrict__ codes,
+                                                       unsigned char* __restrict__ scales, long long steps,
+                                                       long long groups) {
+  constexpr int V = 16 / sizeof(T), LANES = 128 / V, ROWS = 256 / LANES, PASSES = 64 / ROWS;
+  __shared__ unsigned sc[64];
+  const long long step = blockIdx.x % steps, group = blockIdx.x / steps;
+  const int lane = threadIdx.x % LANES, row0 = threadIdx.x / LANES;
+  const long long col = step * 128 + lane * V;
+  if (threadIdx.x < 64) sc[threadIdx.x] = 0;
+  __syncthreads();
+  T raw[PASSES][V];
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const long long row = group * 64 + row0 + p * ROWS;
+    const T* at = src + row * cols + col;
+    if (row < rows && col + V <= cols) {
+      __builtin_memcpy(raw[p], at, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) raw[p][i] = row < rows && col + i < cols ? at[i] : Elem<T>::put(0.0f);
+    }
+  }
+  const long long row_bytes = steps * (FP4 ? 64 : 128);
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int r = row0 + p * ROWS;
+    float v[V];
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      v[i] = Elem<T>::get(raw[p][i]);
+      m = max(m, magnitude<FP4>(v[i]));
+    }
+#pragma unroll
+    for (int d = 1; d < 32 / V; d <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, d, 64));
+    const unsigned byte = FP4 && m >= 0x7f800000u ? 255u : scale_byte<FP4>(m);
+    const float scale = rt_mx::scale_of(min(byte, 254u));
+    unsigned w[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) w[i] = encode4<FP4>(v + 4 * i, scale);
+    if (group * 64 + r < rows) {
+      unsigned char* out = codes + (group * 64 + r) * row_bytes + (step * 128 + lane * V) / (FP4 ? 2 : 1);
+      if constexpr (FP4 && V == 4) *reinterpret_cast<unsigned short*>(out) = (unsigned short)w[0];
+      else if constexpr (FP4) *reinterpret_cast<unsigned*>(out) = w[0] | (w[1] << 16);
+      else if constexpr (V == 4) *reinterpret_cast<unsigned*>(out) = w[0];
+      else *reinterpret_cast<u2*>(out) = u2{w[0], w[1]};
+      if (lane * V % 32 == 0)
+        reinterpret_cast<unsigned char*>(sc)[4 * (16 * (lane * V / 32) + r % 16) + r / 16] = (unsigned char)byte;
+    }
+  }
+  __syncthreads();
+  store_scales(sc, scales, step, groups, group);
+}
+
+// The same of the transpose: src [cols, rows], dst rows of src's columns.  A
+// lane takes one row of dst, a wave 32 of its columns (32 rows of src, each
+// read as 64 consecutive values), so a block's maximum needs no exchange.
+template <typename T, bool FP4>
+__global__ __launch_bounds__(256) void quantize_t_kernel(const T* __restrict__ src, long long rows, long long cols,
+                                                         unsigned char* __restrict__ codes,
+                                                         unsigned char* __restrict__ scales, long long steps,
+                                                         long long groups) {
+  __shared__ unsigned sc[64];
+  const long long group = blockIdx.x % groups, step = blockIdx.x / groups;
+  const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const long long row = group * 64 + lane, col = step * 128 + 32 * g;
+  if (threadIdx.x < 64) sc[threadIdx.x] = 0;
+  __syncthreads();
+  if (row < rows) {
+    T raw[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) raw[i] = col + i < cols ? src[(col + i) * rows + row] : Elem<T>::put(0.0f);
+    float v[32];
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      v[i] = Elem<T>::get(raw[i]);
+      m = max(m, magnitude<FP4>(v[i]));
+    }
+    const unsigned byte = FP4 && m >= 0x7f800000u ? 255u : scale_byte<FP4>(m);
+    const float scale = rt_mx::scale_of(min(byte, 254u));
+    unsigned w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = encode4<FP4>(v + 4 * i, scale);
+    if constexpr (FP4) {
+      u4* out = reinterpret_cast<u4*>(codes + row * (steps * 64) + step * 64 + 16 * g);
+      *out = u4{w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16), w[6] | (w[7] << 16)};
+    } else {
+      u4* out = reinterpret_cast<u4*>(codes + row * (steps * 128) + step * 128 + 32 * g);
+      out[0] = u4{w[0], w[1], w[2], w[3]};
+      out[1] = u4{w[4], w[5], w[6], w[7]};
+    }
+    reinterpret_cast<unsigned char*>(sc)[4 * (16 * g + lane % 16) + lane / 16] = (unsigned char)byte;
+  }
+  __syncthreads();
+  store_scales(sc, scales, step, groups, group);
+}
+
+// Back to values: a lane takes 8 consecutive codes of a row.
+template <typename T, bool FP4>
+__global__ __launch_bounds__(256) void dequantize_kernel(const unsigned char* __restrict__ codes,
+                                                         const unsigned char* __restrict__ scales, T* __restrict__ dst,
+                                                         long long rows, long long cols, long long steps,
+                                                         long long groups) {
+  __shared__ unsigned sc[64];
+  const long long step = blockIdx.x % steps, group = blockIdx.x / steps;
+  const int lane = threadIdx.x % 16, row0 = threadIdx.x / 16;
+  const long long col = step * 128 + lane * 8, row_bytes = steps * (FP4 ? 64 : 128);
+  u2 w[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const long long row = group * 64 + row0 + 16 * p;
+    w[p] = u2{0u, 0u};
+    if (row < rows) {
+      const unsigned char* at = codes + row * row_bytes + col / (FP4 ? 2 : 1);
+      if constexpr (FP4) w[p][0] = *reinterpret_cast<const unsigned*>(at);
+      else w[p] = *reinterpret_cast<const u2*>(at);
+    }
+  }
+  if (threadIdx.x < 64)
+    sc[threadIdx.x] = reinterpret_cast<const unsigned*>(scales)[(step * groups + group) * 64 + threadIdx.x];
+  __syncthreads();
+  // Byte p of a lane's dword is the scale of row row0 + 16 p.
+  const unsigned word = sc[16 * (lane / 4) + row0];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const long long row = group * 64 + row0 + 16 * p;
+    const unsigned byte = (word >> (8 * p)) & 0xffu;
+    const float scale = rt_mx::scale_of(byte);
+    T out[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f2 v;
+      if constexpr (FP4) {
+        if (i == 0) v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[p][0], 1.0f, 0);
+        if (i == 1) v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[p][0], 1.0f, 1);
+        if (i == 2) v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[p][0], 1.0f, 2);
+        if (i == 3) v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[p][0], 1.0f, 3);
+      } else {
+        if (i % 2 == 0) v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[p][i / 2], 1.0f, false);
+        else v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[p][i / 2], 1.0f, true);
+      }
+      out[2 * i] = Elem<T>::put(v[0] * scale);
+      out[2 * i + 1] = Elem<T>::put(v[1] * scale);
+    }
+    if (row >= rows || col >= cols) continue;
+    T* at = dst + row * cols + col;
+    if (col + 8 <= cols) {
+      __builtin_memcpy(at, out, sizeof out);
+    } else {
+      for (int i = 0; i < 8; ++i)
+        if (col + i < cols) at[i] = out[i];
+    }
+  }
+}
+
+// Whether the value converted into this 8-bit code was positive (rt_convert's rule).
+__device__ inline bool positive(unsigned code) { return code == 0x80u || (code >= 1u && code <= 0x7eu); }
+
+// v zeroed where the mask is not positive (VJP false), or v = g · 1[mask > 0]
+// as a product (VJP true: f32).
+template <typename T, bool VJP>
+__global__ __launch_bounds__(256) void mask_kernel(const unsigned char* __restrict__ codes, long long rows,
+                                                   long long cols, long long row_bytes, const T* g, T* v) {
+  const long long chunks = (cols + 3) / 4, n = rows * chunks;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long row = i / chunks, col = 4 * (i - row * chunks);
+    const unsigned w = *reinterpret_cast<const unsigned*>(codes + row * row_bytes + col);
+    T* at = v + row * cols + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (col + e >= cols) break;
+      const bool on = positive((w >> (8 * e)) & 0xffu);
+      if constexpr (VJP) at[e] = g[row * cols + col + e] * (on ? 1.0f : 0.0f);
+      else if (!on) at[e] = Elem<T>::put(0.0f);
+    }
+  }
+}
+
+unsigned grid_for(long long n) {
+  const long long b = (n + 255) / 256;
+  return (unsigned)(b < 1 ? 1 : b > 16384 ? 16384 : b);
+}
+
+template <typename T>
+hipError_t quantize(hipStream_t s, const void* src, bool transposed, const rt::MxTensor& d) {
+  const rt::MxLayout l = rt::mx_layout(d.dtype, d.rows, d.cols);
+  auto* codes = const_cast<unsigned char*>(d.codes);
+  auto* scales = const_cast<unsigned char*>(d.scales);
+  auto go = [&](auto kernel) {
+    rt::launch(kernel, dim3((unsigned)(l.steps * l.groups)), dim3(256), 0, s, static_cast<const T*>(src), d.rows,
+               d.cols, codes, scales, (long long)l.steps, (long long)l.groups);
+  };
+  if (d.dtype == RT_MXFP4) transposed ? go(quantize_t_kernel<T, true>) : go(quantize_kernel<T, true>);
+  else transposed ? go(quantize_t_kernel<T, false>) : go(quantize_kernel<T, false>);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t dequantize(hipStream_t s, const rt::MxTensor& m, void* dst) {
+  const rt::MxLayout l = rt::mx_layout(m.dtype, m.rows, m.cols);
+  auto go = [&](auto kernel) {
+    rt::launch(kernel, dim3((unsigned)(l.steps * l.groups)), dim3(256), 0, s, m.codes, m.scales, static_cast<T*>(dst),
+               m.rows, m.cols, (long long)l.steps, (long long)l.groups);
+  };
+  m.dtype == RT_MXFP4 ? go(dequantize_kernel<T, true>) : go(dequantize_kernel<T, false>);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+namespace rt {
+
+MxTensor mx_tensor(const rt_buf* b) {
+  MxTensor m;
+  m.dtype = b->dtype;
+  m.rows = (long long)b->shape[0];
+  m.cols = (long long)b->shape[1];
+  m.codes = static_cast<const unsigned char*>(b->ptr);
+  m.scales = m.codes + mx_layout(b->dtype, b->shape[0], b->shape[1]).scale_off;
+  return m;
+}
+
+hipError_t mx_quantize_launch(hipStream_t s, const void* src, int src_dtype, bool transposed, const MxTensor& dst) {
+  if (dst.rows == 0 || dst.cols == 0) return hipSuccess;
+  switch (src_dtype) {
+    case RT_F32: return quantize<float>(s, src, transposed, dst);
+    case RT_BF16: return quantize<bf16_bits>(s, src, transposed, dst);
+    case RT_F16: return quantize<_Float16>(s, src, transposed, dst);
+  }
+  return hipErrorInvalidValue;
+}
+
+hipError_t mx_dequantize_launch(hipStream_t s, const MxTensor& src, void* dst, int dst_dtype) {
+  if (src.rows == 0 || src.cols == 0) return hipSuccess;
+  switch (dst_dtype) {
+    case RT_F32: return dequantize<float>(s, src, dst);
+    case RT_BF16: return dequantize<bf16_bits>(s, src, dst);
+    case RT_F16: return dequantize<_Float16>(s, src, dst);
+  }
+  return hipErrorInvalidValue;
+}
+
+hipError_t mx_mask_launch(hipStream_t s, const MxTensor& mask, void* v, int v_dtype) {
+  const long long n = mask.rows * ((mask.cols + 3) / 4);
+  if (n == 0) return hipSuccess;
+  const long long rb = (long long)mx_layout(mask.dtype, mask.rows, mask.cols).row_bytes;
+  if (v_dtype == RT_F32)
+    rt::launch((mask_kernel<float, false>), dim3(grid_for(n)), dim3(256), 0, s, mask.codes, mask.rows, mask.cols, rb,
+               (const float*)nullptr, static_cast<float*>(v));
+  else if (v_dtype == RT_BF16)
+    rt::launch((mask_kernel<bf16_bits, false>), dim3(grid_for(n)), dim3(256), 0, s, mask.codes, mask.rows, mask.cols,
+               rb, (const bf16_bits*)nullptr, static_cast<bf16_bits*>(v));
+  else
+    return hipErrorInvalidValue;
+  return hipGetLastError();
+}
+
+hipError_t mx_relu_vjp_launch(hipStream_t s, const MxTensor& mask, const float* g, float* dx) {
+  const long long n = mask.rows * ((mask.cols + 3) / 4);
+  if (n == 0) return hipSuccess;
+  const long long rb = (long long)mx_layout(mask.dtype, mask.rows, mask.cols).row_bytes;
+  rt::launch((mask_kernel<float, true>), dim3(grid_for(n)), dim3(256), 0, s, mask.codes, mask.rows, mask.cols, rb, g,
+             dx);
+  return hipGetLastError();
+}
+
+}  // namespace rt
+
+// ------------------------------------------------------------------ C ABI
+using namespace rt;
+
+extern "C" int rt_convert_t(rt_ctx* c, const rt_buf* src, rt_buf* dst) {
+  CHECK_CTX(c);
+  if (!src || !dst) return fail(c, RT_ERR_INVALID, "null buffer");
+  if (src->dtype == RT_U32 || is_mx(src->dtype) || !is_mx(dst->dtype))
+    return fail(c, RT_ERR_DTYPE, "convert_t takes f32, bf16 or f16 into a microscaled tensor");
+  if (src->rank != 2 || src->shape[0] != dst->shape[1] || src->shape[1] != dst->shape[0])
+    return fail(c, RT_ERR_SHAPE, "convert_t: the source must be [%zu,%zu]", dst->shape[1], dst->shape[0]);
+  Launch L(c, "convert_t");
+  HIP_TRY(c, mx_quantize_launch(c->stream, src->ptr, src->dtype, true, mx_tensor(dst)), "convert_t");
+  return RT_OK;
+}

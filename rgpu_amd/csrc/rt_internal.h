@@ -21,6 +21,7 @@ struct rt_buf {
   size_t n = 0;      // elements
   size_t bytes = 0;  // n * element size
   size_t cap = 0;    // bytes of the device allocation (its cache size class)
+  bool borrowed = false;  // rt_wrap: the memory is the caller's
 };
 
 struct rt_prof_rec {
@@ -64,7 +65,29 @@ struct rt_ctx {
 namespace rt {
 
 void mlp_release(rt_mlp* p);  // frees the plan's device memory and the struct
-size_t dtype_size(rt_dtype d);
+size_t dtype_size(rt_dtype d);  // bytes of an element; 0 for the microscaled types
+
+// Microscaled tensors (layout in rtensor_hip.h): a step is 128 columns, the K
+// of one scaled MFMA; a group 64 rows, whose scales of a step are one dword a
+// lane.
+inline bool is_mx(int d) { return d == RT_MXFP4 || d == RT_MXFP8; }
+constexpr int kMxBlock = 32, kMxStep = 128, kMxGroup = 64;
+constexpr size_t kMxMaxCols = size_t(1) << 22;  // a tile's row offsets stay below 2^31 bytes
+struct MxLayout {
+  size_t steps, groups;  // of columns, of rows
+  size_t row_bytes;      // codes of a row
+  size_t scale_off;      // bytes from the codes to the scales
+  size_t bytes;
+};
+inline MxLayout mx_layout(int dtype, size_t rows, size_t cols) {
+  MxLayout l;
+  l.steps = (cols + kMxStep - 1) / kMxStep;
+  l.groups = (rows + kMxGroup - 1) / kMxGroup;
+  l.row_bytes = l.steps * (dtype == RT_MXFP4 ? 64 : 128);
+  l.scale_off = (rows * l.row_bytes + 255) & ~size_t(255);
+  l.bytes = rows == 0 || cols == 0 ? 0 : l.scale_off + l.steps * l.groups * 256;
+  return l;
+}
 int fail(rt_ctx* c, int code, const char* fmt, ...);
 int hip_fail(rt_ctx* c, hipError_t e, const char* what);
 // Makes c->scratch hold at least elems floats (grow-only; waits for queued
@@ -255,6 +278,32 @@ hipError_t head_xent_launch(hipStream_t s, const float* A, int K, const float* W
 hipError_t argmax_launch(hipStream_t s, const float* z, uint32_t* out, int rows, int cols);
 hipError_t convert_launch(hipStream_t s, const void* src, int src_dtype, void* dst, int dst_dtype, size_t n);
 hipError_t fill_i32_launch(hipStream_t s, int* p, int v, size_t n);
+
+// ---------------------------------------------------------------- microscaled (mx.hip, mx_gemm.hip, mx_backward.hip)
+// A microscaled operand: its codes, the scales mx_layout().scale_off behind
+// them, and its shape.
+struct MxTensor {
+  int dtype = RT_MXFP4;
+  const unsigned char* codes = nullptr;
+  const unsigned char* scales = nullptr;
+  long long rows = 0, cols = 0;
+};
+MxTensor mx_tensor(const rt_buf* b);
+// src f32/bf16/f16 [rows, cols] -> dst, or with transposed [cols, rows] -> dst [rows, cols].
+hipError_t mx_quantize_launch(hipStream_t s, const void* src, int src_dtype, bool transposed, const MxTensor& dst);
+hipError_t mx_dequantize_launch(hipStream_t s, const MxTensor& src, void* dst, int dst_dtype);
+// v (f32 or bf16, the mask's shape) zeroed where the mask is not positive.
+hipError_t mx_mask_launch(hipStream_t s, const MxTensor& mask, void* v, int v_dtype);
+// dx = g · 1[mask > 0], as a product (the VJP of the tape's ReLU).
+hipError_t mx_relu_vjp_launch(hipStream_t s, const MxTensor& mask, const float* g, float* dx);
+// C [M, N] = A·Bᵀ with A [M, K] and B RT_MXFP4 [N, K]; epi none, bias or bias and ReLU.
+hipError_t mx_gemm_launch(hipStream_t s, const MxTensor& a, const MxTensor& b, void* C, int out_dtype, int epi,
+                          const float* bias);
+// C [K, N] (f32) = Xᵀ·δ with X RT_MXFP8 [rows, K] and δ [rows, N]; scratch holds
+// mx_dw_scratch_elems floats.
+size_t mx_dw_scratch_elems(const MxTensor& x, int delta_dtype, long long N);
+hipError_t mx_dw_launch(hipStream_t s, const MxTensor& x, const void* delta, int delta_dtype, long long N, float* C,
+                        float* scratch);
 
 // ---------------------------------------------------------------- optimizer
 struct OptTensor {

@@ -26,6 +26,8 @@ size_t dtype_size(rt_dtype d) {
     case RT_BF16: return 2;
     case RT_F16: return 2;
     case RT_U32: return 4;
+    case RT_MXFP4:
+    case RT_MXFP8: return 0;
   }
   return 0;
 }
@@ -172,7 +174,7 @@ int rt_close(rt_ctx* c) {
   for (rt_mlp* p : c->mlps) mlp_release(p);
   c->mlps.clear();
   for (rt_buf* b : c->bufs) {
-    if (b->ptr) hipFree(b->ptr);
+    if (b->ptr && !b->borrowed) hipFree(b->ptr);
     delete b;
   }
   c->bufs.clear();
@@ -264,21 +266,51 @@ static void pool_release(rt_ctx* c, void* ptr, size_t cap) {
   c->pool_bytes += cap;
 }
 
-static int make_buf(rt_ctx* c, rt_dtype dtype, const size_t* shape, int rank, rt_buf** out) {
-  if (out == nullptr || (rank > 0 && shape == nullptr) || rank < 0 || rank > 4)
-    return fail(c, RT_ERR_INVALID, "bad shape arguments");
-  if (dtype < RT_F32 || dtype > RT_U32) return fail(c, RT_ERR_DTYPE, "unknown dtype %d", (int)dtype);
+// A buffer's record without memory: dtype and shape checked, sizes computed.
+static int describe_buf(rt_dtype dtype, const size_t* shape, int rank, rt_buf* b, const char** why) {
+  if ((rank > 0 && shape == nullptr) || rank < 0 || rank > 4) {
+    *why = "bad shape arguments";
+    return RT_ERR_INVALID;
+  }
+  if (dtype < RT_F32 || dtype > RT_MXFP8) {
+    *why = "unknown dtype";
+    return RT_ERR_DTYPE;
+  }
   size_t n = 1;
   for (int i = 0; i < rank; ++i) {
-    if (shape[i] != 0 && n > (SIZE_MAX >> 4) / shape[i]) return fail(c, RT_ERR_SHAPE, "shape too large");
+    if (shape[i] != 0 && n > (SIZE_MAX >> 4) / shape[i]) {
+      *why = "shape too large";
+      return RT_ERR_SHAPE;
+    }
     n *= shape[i];
   }
-  auto* b = new rt_buf();
   b->dtype = dtype;
   b->rank = rank;
   for (int i = 0; i < rank; ++i) b->shape[i] = shape[i];
   b->n = n;
   b->bytes = n * dtype_size(dtype);
+  if (is_mx(dtype)) {
+    if (rank != 2) {
+      *why = "microscaled tensors have rank 2";
+      return RT_ERR_SHAPE;
+    }
+    // Rows and steps are counted in int; padding a row multiplies its bytes by
+    // 128 at most.
+    if (shape[0] > kRowOpMax || shape[1] > kRowOpMax) {
+      *why = "microscaled tensor too large";
+      return RT_ERR_SHAPE;
+    }
+    b->bytes = mx_layout(dtype, shape[0], shape[1]).bytes;
+  }
+  return RT_OK;
+}
+
+static int make_buf(rt_ctx* c, rt_dtype dtype, const size_t* shape, int rank, rt_buf** out) {
+  if (out == nullptr) return fail(c, RT_ERR_INVALID, "bad shape arguments");
+  rt_buf d;
+  const char* why = "";
+  if (int rc = describe_buf(dtype, shape, rank, &d, &why)) return fail(c, rc, "%s (dtype %d)", why, (int)dtype);
+  auto* b = new rt_buf(d);
   if (b->bytes > 0) {
     // Whole 256-byte granules, so fills and vector loads never need a tail.
     b->cap = size_class(b->bytes);
@@ -296,8 +328,48 @@ static int make_buf(rt_ctx* c, rt_dtype dtype, const size_t* shape, int rank, rt
 // Undoes make_buf for a buffer whose initialisation failed.
 static void drop_buf(rt_ctx* c, rt_buf* b) {
   c->bufs.erase(b);
-  pool_release(c, b->ptr, b->cap);
+  if (!b->borrowed) pool_release(c, b->ptr, b->cap);
   delete b;
+}
+
+size_t rt_tensor_bytes(rt_dtype dtype, const size_t* shape, int rank) {
+  rt_buf d;
+  const char* why = "";
+  return describe_buf(dtype, shape, rank, &d, &why) == RT_OK ? d.bytes : 0;
+}
+
+int rt_wrap(rt_ctx* c, rt_dtype dtype, const size_t* shape, int rank, void* ptr, rt_buf** out) {
+  CHECK_CTX(c);
+  if (out == nullptr) return fail(c, RT_ERR_INVALID, "bad shape arguments");
+  *out = nullptr;
+  rt_buf d;
+  const char* why = "";
+  if (int rc = describe_buf(dtype, shape, rank, &d, &why)) return fail(c, rc, "%s (dtype %d)", why, (int)dtype);
+  if (d.bytes > 0) {
+    if (ptr == nullptr) return fail(c, RT_ERR_INVALID, "null device pointer");
+    const size_t align = is_mx(dtype) ? 16 : dtype_size(dtype);
+    if (reinterpret_cast<uintptr_t>(ptr) % align != 0)
+      return fail(c, RT_ERR_INVALID, "the pointer is not aligned to %zu bytes", align);
+    hipPointerAttribute_t at;
+    hipError_t e = hipPointerGetAttributes(&at, ptr);
+    if (e != hipSuccess || at.type != hipMemoryTypeDevice || at.device != c->device) {
+      (void)hipGetLastError();
+      return fail(c, RT_ERR_INVALID, "the pointer is not memory of device %d", c->device);
+    }
+    hipDeviceptr_t base = nullptr;
+    size_t size = 0;
+    HIP_TRY(c, hipMemGetAddressRange(&base, &size, ptr), "address range");
+    const size_t before = static_cast<char*>(ptr) - static_cast<char*>(base);
+    if (before > size || d.bytes > size - before)
+      return fail(c, RT_ERR_SHAPE, "the tensor has %zu bytes, its memory %zu from the pointer on", d.bytes,
+                  before > size ? 0 : size - before);
+    d.ptr = ptr;
+  }
+  d.borrowed = true;
+  auto* b = new rt_buf(d);
+  c->bufs.insert(b);
+  *out = b;
+  return RT_OK;
 }
 
 int rt_zeros(rt_ctx* c, rt_dtype dtype, const size_t* shape, int rank, rt_buf** out) {
@@ -401,6 +473,20 @@ int rt_convert(rt_ctx* c, const rt_buf* src, rt_buf* dst) {
   if (!src || !dst) return fail(c, RT_ERR_INVALID, "null buffer");
   if (src->n != dst->n) return fail(c, RT_ERR_SHAPE, "convert: %zu vs %zu elements", src->n, dst->n);
   if (src->dtype == RT_U32 || dst->dtype == RT_U32) return fail(c, RT_ERR_DTYPE, "convert: u32 not supported");
+  if (is_mx(src->dtype) || is_mx(dst->dtype)) {
+    if (is_mx(src->dtype) && is_mx(dst->dtype))
+      return fail(c, RT_ERR_DTYPE, "convert: one side must be f32, bf16 or f16");
+    if (src->rank != 2 || dst->rank != 2 || src->shape[0] != dst->shape[0] || src->shape[1] != dst->shape[1])
+      return fail(c, RT_ERR_SHAPE, "convert: a microscaled tensor and its values have the same shape");
+    if (is_mx(dst->dtype)) {
+      Launch L(c, "quantize");
+      HIP_TRY(c, mx_quantize_launch(c->stream, src->ptr, src->dtype, false, mx_tensor(dst)), "quantize");
+    } else {
+      Launch L(c, "dequantize");
+      HIP_TRY(c, mx_dequantize_launch(c->stream, mx_tensor(src), dst->ptr, dst->dtype), "dequantize");
+    }
+    return RT_OK;
+  }
   Launch L(c, "convert");
   HIP_TRY(c, convert_launch(c->stream, src->ptr, src->dtype, dst->ptr, dst->dtype, src->n), "convert");
   return RT_OK;
@@ -432,10 +518,58 @@ static int check_epilogue(rt_ctx* c, rt_epilogue epi, const rt_buf* aux, const r
     if (aux->dtype != RT_F32 || aux->n != N) return fail(c, RT_ERR_SHAPE, "bias must be f32 with %zu elements", N);
   } else if (epi == RT_EPI_RELU_MASK) {
     if (aux->n != M * N || aux->dtype == RT_U32) return fail(c, RT_ERR_SHAPE, "mask must match C [%zu,%zu]", M, N);
+    if (aux->dtype == RT_MXFP8) {
+      if (aux->shape[0] != M || aux->shape[1] != N) return fail(c, RT_ERR_SHAPE, "mask must match C [%zu,%zu]", M, N);
+      return RT_OK;
+    }
     if (aux->dtype != out->dtype && !(out->dtype == RT_F32 && aux->dtype == RT_F32))
       return fail(c, RT_ERR_DTYPE, "mask dtype must match C");
   } else {
     return fail(c, RT_ERR_INVALID, "unknown epilogue %d", (int)epi);
+  }
+  return RT_OK;
+}
+
+// rt_gemm with a microscaled operand; shapes and C's size are checked.
+static int mx_gemm(rt_ctx* c, rt_layout layout, const rt_buf* a, const rt_buf* b, rt_buf* out, rt_epilogue epi,
+                   const rt_buf* aux, rt_buf* colsum, size_t M, size_t N, size_t K) {
+  int rc;
+  if (layout == RT_NT && is_mx(a->dtype) && b->dtype == RT_MXFP4) {
+    if (K > kMxMaxCols) return fail(c, RT_ERR_SHAPE, "K of a microscaled product is at most 2^22");
+    if (out->dtype != RT_F32 && out->dtype != RT_BF16) return fail(c, RT_ERR_DTYPE, "microscaled GEMM writes f32 or bf16");
+    if (epi != RT_EPI_NONE && epi != RT_EPI_BIAS && epi != RT_EPI_BIAS_RELU)
+      return fail(c, RT_ERR_INVALID, "microscaled GEMM: no such epilogue %d", (int)epi);
+    if ((rc = check_epilogue(c, epi, aux, out, M, N))) return rc;
+    if (colsum) return fail(c, RT_ERR_INVALID, "fused colsum is only for the TN layout");
+    if (M == 0 || N == 0) return RT_OK;
+    Launch L(c, "mx_gemm_nt");
+    HIP_TRY(c,
+            mx_gemm_launch(c->stream, mx_tensor(a), mx_tensor(b), out->ptr, out->dtype, epi,
+                           aux ? static_cast<const float*>(aux->ptr) : nullptr),
+            "microscaled gemm");
+    return RT_OK;
+  }
+  if (layout != RT_TN || a->dtype != RT_MXFP8 || is_mx(b->dtype) || b->dtype == RT_U32)
+    return fail(c, RT_ERR_DTYPE, "microscaled operands: NT with a 4-bit B, or TN of an 8-bit A and an f32, bf16 or f16 B");
+  if (out->dtype != RT_F32) return fail(c, RT_ERR_DTYPE, "the gradient from an 8-bit input is f32");
+  if (epi != RT_EPI_NONE) return fail(c, RT_ERR_INVALID, "the TN product of an 8-bit A has no epilogue");
+  if (colsum && (colsum->dtype != RT_F32 || colsum->n != N)) return fail(c, RT_ERR_SHAPE, "colsum must be f32 [%zu]", N);
+  if (N == 0) return RT_OK;
+  const MxTensor x = mx_tensor(a);
+  if ((rc = ensure_scratch(c, std::max(mx_dw_scratch_elems(x, b->dtype, (long long)N),
+                                       colsum ? colsum_scratch_elems((int)K, (int)N, b->dtype) : 0))))
+    return rc;
+  if (M > 0) {
+    Launch L(c, "mx_gemm_tn");
+    HIP_TRY(c, mx_dw_launch(c->stream, x, b->ptr, b->dtype, (long long)N, static_cast<float*>(out->ptr), c->scratch),
+            "gradient from an 8-bit input");
+  }
+  if (colsum) {
+    Launch L(c, "colsum");
+    HIP_TRY(c,
+            colsum_launch(c->stream, b->ptr, b->dtype, (int)K, (int)N, static_cast<float*>(colsum->ptr), c->scratch,
+                          c->scratch_elems),
+            "colsum");
   }
   return RT_OK;
 }
@@ -449,6 +583,7 @@ int rt_gemm(rt_ctx* c, rt_layout layout, const rt_buf* a, const rt_buf* b, rt_bu
   if (rc) return rc;
   if (out->n != M * N || (out->rank == 2 && (out->shape[0] != M || out->shape[1] != N)))
     return fail(c, RT_ERR_SHAPE, "C must be [%zu,%zu]", M, N);
+  if (is_mx(a->dtype) || is_mx(b->dtype)) return mx_gemm(c, layout, a, b, out, epi, aux, colsum, M, N, K);
   if (a->dtype != b->dtype || a->dtype == RT_U32) return fail(c, RT_ERR_DTYPE, "A and B must share a float dtype");
   if (a->dtype == RT_F32 && out->dtype != RT_F32) return fail(c, RT_ERR_DTYPE, "f32 GEMM writes f32");
   if (is_half(a->dtype) && !(out->dtype == RT_F32 || out->dtype == RT_BF16))
@@ -459,6 +594,13 @@ int rt_gemm(rt_ctx* c, rt_layout layout, const rt_buf* a, const rt_buf* b, rt_bu
     if (colsum->dtype != RT_F32 || colsum->n != N) return fail(c, RT_ERR_SHAPE, "colsum must be f32 [%zu]", N);
   }
   if (M == 0 || N == 0) return RT_OK;
+  if (epi == RT_EPI_RELU_MASK && aux->dtype == RT_MXFP8) {
+    // The product as it stands, then the mask.
+    if ((rc = rt_gemm(c, layout, a, b, out, RT_EPI_NONE, nullptr, colsum))) return rc;
+    Launch L(c, "mx_mask");
+    HIP_TRY(c, mx_mask_launch(c->stream, mx_tensor(aux), out->ptr, out->dtype), "mask");
+    return RT_OK;
+  }
   GemmDesc d;
   d.layout = layout;
   d.in_dtype = a->dtype;
@@ -569,7 +711,8 @@ int splitk_check(rt_ctx* c, rt_layout layout, const rt_buf* a, const rt_buf* b, 
   int rc = gemm_shapes(c, layout, a, b, M, N, K);
   if (rc) return rc;
   if (out->n != *M * *N || out->dtype != RT_F32) return fail(c, RT_ERR_SHAPE, "C must be f32 [%zu,%zu]", *M, *N);
-  if (a->dtype != b->dtype || a->dtype == RT_U32) return fail(c, RT_ERR_DTYPE, "A and B must share a float dtype");
+  if (a->dtype != b->dtype || a->dtype == RT_U32 || is_mx(a->dtype))
+    return fail(c, RT_ERR_DTYPE, "A and B must share a float dtype");
   if (colsum) {
     if (layout != RT_TN) return fail(c, RT_ERR_INVALID, "fused colsum is only for the TN layout");
     if (colsum->dtype != RT_F32 || colsum->n != *N) return fail(c, RT_ERR_SHAPE, "colsum must be f32 [%zu]", *N);
@@ -666,6 +809,7 @@ int rt_colsum(rt_ctx* c, const rt_buf* src, rt_buf* dst) {
   size_t R = src->shape[0], Cc = src->shape[1];
   if (dst->dtype != RT_F32 || dst->n != Cc) return fail(c, RT_ERR_SHAPE, "colsum target must be f32 [1,%zu]", Cc);
   if (src->dtype == RT_U32) return fail(c, RT_ERR_DTYPE, "colsum of u32");
+  if (is_mx(src->dtype)) return fail(c, RT_ERR_DTYPE, "colsum of a microscaled tensor");
   if (R > kRowOpMax || Cc > kRowOpMax) return fail(c, RT_ERR_SHAPE, "colsum source too large");
   int rc = ensure_scratch(c, colsum_scratch_elems((int)R, (int)Cc, src->dtype));
   if (rc) return rc;
@@ -706,8 +850,15 @@ int rt_relu_bwd(rt_ctx* c, const rt_buf* a, rt_buf* delta) {
   if (!a || !delta) return fail(c, RT_ERR_INVALID, "null buffer");
   if (delta->dtype != RT_F32 || a->dtype == RT_U32 || a->n != delta->n)
     return fail(c, RT_ERR_SHAPE, "relu_bwd: delta f32, same size as a");
+  if (a->dtype == RT_MXFP4) return fail(c, RT_ERR_DTYPE, "relu_bwd: a 4-bit activation keeps no mask");
+  if (a->dtype == RT_MXFP8 && (delta->rank != 2 || delta->shape[0] != a->shape[0] || delta->shape[1] != a->shape[1]))
+    return fail(c, RT_ERR_SHAPE, "relu_bwd: delta must be [%zu,%zu]", a->shape[0], a->shape[1]);
   if (a->n == 0) return RT_OK;
   Launch L(c, "relu_bwd");
+  if (a->dtype == RT_MXFP8) {
+    HIP_TRY(c, mx_mask_launch(c->stream, mx_tensor(a), delta->ptr, RT_F32), "relu_bwd");
+    return RT_OK;
+  }
   HIP_TRY(c, relu_bwd_launch(c->stream, a->ptr, a->dtype, static_cast<float*>(delta->ptr), a->n), "relu_bwd");
   return RT_OK;
 }

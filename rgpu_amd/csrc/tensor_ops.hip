@@ -910,10 +910,20 @@ int rt_map_vjp(rt_ctx* c, rt_unary_op op, float k, const rt_buf* g, const rt_buf
   if (op < RT_U_SCALE || op > RT_U_TANH) return fail(c, RT_ERR_INVALID, "unknown unary op %d", (int)op);
   if (needs_x(op) && !x) return fail(c, RT_ERR_INVALID, "this VJP needs the op's input");
   if (needs_y(op) && !y) return fail(c, RT_ERR_INVALID, "this VJP needs the op's output");
-  if (!is_f32(g) || !is_f32(dx) || (x && !is_f32(x)) || (y && !is_f32(y))) return fail(c, RT_ERR_DTYPE, "f32 only");
+  const bool saved8 = op == RT_U_RELU && x->dtype == RT_MXFP8;  // the activation as it was saved in 8 bits
+  if (!is_f32(g) || !is_f32(dx) || (x && !is_f32(x) && !saved8) || (y && !is_f32(y)))
+    return fail(c, RT_ERR_DTYPE, "f32 only");
   if (g->n != dx->n || (x && x->n != g->n) || (y && y->n != g->n))
     return fail(c, RT_ERR_SHAPE, "map_vjp: operands differ in size");
+  if (saved8 && (g->rank != 2 || g->shape[0] != x->shape[0] || g->shape[1] != x->shape[1]))
+    return fail(c, RT_ERR_SHAPE, "map_vjp: g must be [%zu,%zu]", x->shape[0], x->shape[1]);
   Launch L(c, "map_vjp");
+  if (saved8) {
+    HIP_TRY(c,
+            mx_relu_vjp_launch(c->stream, mx_tensor(x), static_cast<const float*>(g->ptr), static_cast<float*>(dx->ptr)),
+            "map_vjp");
+    return RT_OK;
+  }
   HIP_TRY(c,
           unary_vjp_launch(c->stream, op, k, static_cast<const float*>(g->ptr),
                            needs_x(op) ? static_cast<const float*>(x->ptr) : nullptr,

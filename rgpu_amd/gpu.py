@@ -40,6 +40,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "librtensor_hip.so")
 
 F32, BF16, F16, U32 = 0, 1, 2, 3
+MXFP4, MXFP8 = 4, 5  # microscaled 4-bit and 8-bit floating point (include/rtensor_hip.h)
 NN, TN, NT = 0, 1, 2
 EPI_NONE, EPI_BIAS, EPI_BIAS_RELU, EPI_RELU_MASK = 0, 1, 2, 3
 OPT_ADAM, OPT_SGD = 0, 1
@@ -69,7 +70,10 @@ SIGNATURES = {
     "rt_free": (C.c_int, [_VP, _VP]),
     "rt_buf_info": (C.c_int, [_VP, C.POINTER(C.c_int), _SZP, C.POINTER(C.c_int)]),
     "rt_upload_labels": (C.c_int, [_VP, C.POINTER(C.c_uint64), C.c_size_t, C.POINTER(_VP)]),
+    "rt_wrap": (C.c_int, [_VP, C.c_int, _SZP, C.c_int, _VP, C.POINTER(_VP)]),
+    "rt_tensor_bytes": (C.c_size_t, [C.c_int, _SZP, C.c_int]),
     "rt_convert": (C.c_int, [_VP, _VP, _VP]),
+    "rt_convert_t": (C.c_int, [_VP, _VP, _VP]),
     "rt_gemm": (C.c_int, [_VP, C.c_int, _VP, _VP, _VP, C.c_int, _VP, _VP]),
     "rt_gemm_splitk": (C.c_int, [_VP, C.c_int, _VP, _VP, _VP, _VP, C.c_size_t, _VP]),
     "rt_gemm_splitk_static": (C.c_int, [_VP, C.c_int, _VP, _VP, _VP, C.c_size_t, _VP]),
@@ -165,6 +169,40 @@ def _np_dtype(dt: int):
 _ITEMSIZE = {F32: 4, BF16: 2, F16: 2, U32: 4}
 
 
+def tensor_bytes(shape, dtype: int) -> int:
+    """Bytes of a tensor on the device (rt_tensor_bytes)."""
+    if dtype in _ITEMSIZE:
+        return math.prod(shape) * _ITEMSIZE[dtype]
+    return int(lib().rt_tensor_bytes(dtype, (C.c_size_t * max(len(shape), 1))(*shape), len(shape)))
+
+
+def mx_decode(data, shape, dtype: int) -> np.ndarray:
+    """The f32 values of a microscaled tensor's bytes (what ``Gpu.download`` gives for one), on the host."""
+    rows, cols = shape
+    data = np.ascontiguousarray(data, dtype=np.uint8).reshape(-1)
+    steps, groups = -(-cols // 128), -(-rows // 64)
+    row_bytes = steps * (64 if dtype == MXFP4 else 128)
+    at = -(-rows * row_bytes // 256) * 256
+    code = data[:rows * row_bytes].reshape(rows, row_bytes)
+    if dtype == MXFP4:
+        code = np.stack([code & 15, code >> 4], axis=2).reshape(rows, -1)
+        value = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6], np.float32)[code & 7]
+        negative = code >= 8
+    else:
+        e, m = ((code >> 3) & 15).astype(np.int32), (code & 7).astype(np.float32)
+        value = np.where(e == 0, np.ldexp(m, -9), np.ldexp(8 + m, e - 10)).astype(np.float32)
+        value[(code & 0x7F) == 0x7F] = np.nan
+        negative = code >= 128
+    value = np.where(negative, -value, value)
+    # [step, group, g, r, t] -> row 64 group + 16 t + r, block 4 step + g
+    scale = data[at:at + steps * groups * 256].reshape(steps, groups, 4, 16, 4).transpose(1, 4, 3, 0, 2)
+    scale = scale.reshape(groups * 64, steps * 4)[:rows].astype(np.int32)
+    factor = np.where(scale == 255, np.float32(np.nan), np.ldexp(np.float32(1), np.minimum(scale, 254) - 127))
+    with np.errstate(over="ignore"):  # an MXFP4 element from 2^128 on
+        out = value.reshape(rows, -1, 32) * factor.astype(np.float32)[:, :, None]
+    return out.reshape(rows, -1)[:, :cols]
+
+
 def _shape(shape) -> tuple:
     """A shape as a tuple of Python ints (the common case passes through)."""
     if type(shape) is tuple and all(type(d) is int for d in shape):
@@ -186,9 +224,11 @@ def bf16_bits_to_f32(b) -> np.ndarray:
 
 
 class GpuTensor:
-    """``GpuTensor`` (mod.rs:190-208): owns one device buffer."""
+    """``GpuTensor`` (mod.rs:190-208): owns one device buffer (``Gpu.wrap``:
+    a handle on memory that ``owner`` keeps)."""
 
-    def __init__(self, gpu: "Gpu", handle: int, shape, dtype: int):
+    def __init__(self, gpu: "Gpu", handle: int, shape, dtype: int, owner=None, wrapped: bool = False):
+        self.owner, self.wrapped = owner, wrapped
         self.gpu = gpu
         self.handle = handle
         self.shape = _shape(shape)
@@ -205,6 +245,11 @@ class GpuTensor:
         if self.handle and self.gpu._h and not self.gpu._keep(self):
             self.gpu._call("rt_free", self.gpu._h, self.handle)
         self.handle = None
+        self.owner = None
+
+    @property
+    def nbytes(self) -> int:
+        return tensor_bytes(self.shape, self.dtype)
 
     def __del__(self):
         try:
@@ -234,7 +279,7 @@ class Gpu:
     _SPARE_MAX_BYTES = 64 << 20
 
     def _keep(self, t: "GpuTensor") -> bool:
-        if len(t) * _ITEMSIZE[t.dtype] > self._SPARE_MAX_BYTES:
+        if t.wrapped or t.nbytes > self._SPARE_MAX_BYTES:
             return False
         lst = self._spare.setdefault((t.shape, t.dtype), [])
         if len(lst) >= self._SPARE_PER_SHAPE:
@@ -288,11 +333,31 @@ class Gpu:
         self._call("rt_empty", self._h, dtype, arr, len(shape), C.byref(h))
         return GpuTensor(self, h.value, shape, dtype)
 
-    def upload(self, a, dtype: Optional[int] = None) -> GpuTensor:
+    def wrap(self, ptr: int, shape, dtype: int = F32, owner=None) -> GpuTensor:
+        """A tensor over device memory that something else owns (rt_wrap),
+        such as ``t.data_ptr()`` of a contiguous torch tensor t on this device.
+        ``owner`` is kept as long as the handle.  Order the context's stream
+        against others that use the memory (``sync``, a device
+        synchronisation)."""
+        shape = _shape(shape)
+        arr = (C.c_size_t * max(len(shape), 1))(*shape)
+        h = C.c_void_p()
+        self._call("rt_wrap", self._h, dtype, arr, len(shape), C.c_void_p(ptr), C.byref(h))
+        return GpuTensor(self, h.value, shape, dtype, owner, True)
+
+    def upload(self, a, dtype: Optional[int] = None, shape=None) -> GpuTensor:
         """Upload a host array.  dtype BF16 takes f32 values (rounded to
         nearest even) or uint16 bit patterns; F16 takes anything numpy can
-        cast to float16."""
+        cast to float16; MXFP4 and MXFP8 take the bytes of a tensor of
+        ``shape`` as ``download`` gives them."""
         a = np.asarray(a)
+        if dtype in (MXFP4, MXFP8):
+            host, shape = np.ascontiguousarray(a, dtype=np.uint8), _shape(shape)
+            if host.nbytes != tensor_bytes(shape, dtype):
+                raise ValueError(f"a tensor {shape} has {tensor_bytes(shape, dtype)} bytes, got {host.nbytes}")
+            arr, h = (C.c_size_t * max(len(shape), 1))(*shape), C.c_void_p()
+            self._call("rt_upload", self._h, dtype, arr, len(shape), host.ctypes.data_as(C.c_void_p), C.byref(h))
+            return GpuTensor(self, h.value, shape, dtype)
         if dtype is None:
             dtype = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.uint32): U32}.get(a.dtype, F32)
         if dtype == BF16:
@@ -307,7 +372,7 @@ class Gpu:
         return GpuTensor(self, h.value, shape, dtype)
 
     def download(self, t: GpuTensor) -> np.ndarray:
-        out = np.empty(t.shape, _np_dtype(t.dtype))
+        out = np.empty(t.nbytes, np.uint8) if t.dtype in (MXFP4, MXFP8) else np.empty(t.shape, _np_dtype(t.dtype))
         self._call("rt_download", self._h, t.handle, out.ctypes.data_as(C.c_void_p), out.nbytes)
         return out
 
@@ -315,14 +380,23 @@ class Gpu:
         a = self.download(t)
         if t.dtype == BF16:
             return bf16_bits_to_f32(a)
+        if t.dtype in (MXFP4, MXFP8):
+            return mx_decode(a, t.shape, t.dtype)
         return a.astype(np.float32)
 
     def write(self, t: GpuTensor, a) -> None:
-        host = np.ascontiguousarray(a, dtype=_np_dtype(t.dtype))
+        host = np.ascontiguousarray(a, dtype=np.uint8 if t.dtype in (MXFP4, MXFP8) else _np_dtype(t.dtype))
         self._call("rt_write", self._h, t.handle, host.ctypes.data_as(C.c_void_p), host.nbytes)
 
     def convert(self, src: GpuTensor, dst: GpuTensor) -> None:
+        """f32/bf16/f16 into each other, and to or from MXFP4/MXFP8 (blocks of
+        32 along the rows)."""
         self._call("rt_convert", self._h, src.handle, dst.handle)
+
+    def convert_t(self, src: GpuTensor, dst: GpuTensor) -> None:
+        """The transpose of src [R, C] into the MXFP4/MXFP8 tensor dst [C, R]:
+        a weight [in, out] as the B of ``gemm(NT, ...)``."""
+        self._call("rt_convert_t", self._h, src.handle, dst.handle)
 
     # --------------------------------------------------------------- ops
     def gemm(self, layout: int, a: GpuTensor, b: GpuTensor, c: GpuTensor, epi: int = EPI_NONE,

@@ -1,0 +1,444 @@
+"""Microscaled tensors on the device against numpy in 64 bits (tests/mx_common.py): conversion to the byte, the products
+within the rounding of their sums, the mask exactly, and what is refused."""
+import numpy as np
+import pytest
+import torch
+
+from rgpu_amd import gpu as G
+from tests import mx_common as X
+
+pytestmark = pytest.mark.gpu
+
+FMT = {"fp4": G.MXFP4, "fp8": G.MXFP8}
+DTYPE = {"f32": G.F32, "bf16": G.BF16, "f16": G.F16}
+
+
+@pytest.fixture(scope="module")
+def gpu():
+    g = G.Gpu(0)
+    yield g
+    g.close()
+
+
+def status(call, *args, **kw):
+    with pytest.raises(G.RtError) as e:
+        call(*args, **kw)
+    return e.value.status
+
+
+def rounded(x, dtype):
+    """x as the type holds it, in f64."""
+    if dtype == G.BF16:
+        return G.bf16_bits_to_f32(G.f32_to_bf16_bits(x)).astype(np.float64)
+    if dtype == G.F16:
+        return np.asarray(x, np.float32).astype(np.float16).astype(np.float64)
+    return np.asarray(x, np.float32).astype(np.float64)
+
+
+def mx_upload(gpu, x, fmt):
+    code, byte, values = X.quantize(x, fmt)
+    return gpu.upload(X.pack(code, byte, fmt), fmt, x.shape), values
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals(gpu):
+    f = lambda *s: gpu.zeros(s)
+    m4, m8 = gpu.zeros((8, 40), G.MXFP4), gpu.zeros((8, 40), G.MXFP8)
+    u = gpu.zeros((8, 40), G.U32)
+    assert status(gpu.zeros, (8,), G.MXFP4) == "RT_ERR_SHAPE"
+    assert status(gpu.zeros, (2, 8, 40), G.MXFP8) == "RT_ERR_SHAPE"
+    assert status(gpu.zeros, (2 ** 31, 1), G.MXFP8) == "RT_ERR_SHAPE"
+    assert status(gpu.zeros, (8, 40), 6) == "RT_ERR_DTYPE"
+    assert status(gpu.convert, u, m4) == "RT_ERR_DTYPE"
+    assert status(gpu.convert, m4, m8) == "RT_ERR_DTYPE"
+    assert status(gpu.convert, f(40, 8), m4) == "RT_ERR_SHAPE"
+    assert status(gpu.convert, f(320), m4) == "RT_ERR_SHAPE"
+    assert status(gpu.convert_t, f(8, 40), m4) == "RT_ERR_SHAPE"
+    assert status(gpu.convert_t, f(320), m4) == "RT_ERR_SHAPE"
+    assert status(gpu.convert_t, m8, m4) == "RT_ERR_DTYPE"
+    assert status(gpu.convert_t, u, m4) == "RT_ERR_DTYPE"
+    assert status(gpu.convert_t, f(40, 8), f(8, 40)) == "RT_ERR_DTYPE"
+    # products
+    c = f(8, 8)
+    assert status(gpu.gemm, G.NN, m4, gpu.zeros((40, 8), G.MXFP4), c) == "RT_ERR_DTYPE"
+    assert status(gpu.gemm, G.NT, m4, f(8, 40), c) == "RT_ERR_DTYPE"
+    assert status(gpu.gemm, G.NT, m4, m8, c) == "RT_ERR_DTYPE"
+    assert status(gpu.gemm, G.NT, m8, m8, c) == "RT_ERR_DTYPE"
+    assert status(gpu.gemm, G.NT, f(8, 40), m4, c) == "RT_ERR_DTYPE"
+    assert status(gpu.gemm, G.NT, m4, gpu.zeros((8, 41), G.MXFP4), c) == "RT_ERR_SHAPE"
+    assert status(gpu.gemm, G.NT, m4, m4, f(8, 9)) == "RT_ERR_SHAPE"
+    assert status(gpu.gemm, G.NT, m4, m4, gpu.zeros((8, 8), G.F16)) == "RT_ERR_DTYPE"
+    assert status(gpu.gemm, G.NT, m4, m4, gpu.zeros((8, 8), G.MXFP8)) == "RT_ERR_DTYPE"
+    assert status(gpu.gemm, G.NT, m4, m4, c, G.EPI_RELU_MASK, f(8, 8)) == "RT_ERR_INVALID"
+    assert status(gpu.gemm, G.NT, m4, m4, c, G.EPI_BIAS, f(1, 9)) == "RT_ERR_SHAPE"
+    assert status(gpu.gemm, G.NT, m4, m4, c, G.EPI_BIAS) == "RT_ERR_INVALID"
+    assert status(gpu.gemm, G.NT, m4, m4, c, colsum=f(8)) == "RT_ERR_INVALID"
+    dw = f(40, 8)
+    assert status(gpu.matmul_at_b, m4, f(8, 8), dw) == "RT_ERR_DTYPE"
+    assert status(gpu.matmul_at_b, m8, gpu.zeros((8, 8), G.U32), dw) == "RT_ERR_DTYPE"
+    assert status(gpu.matmul_at_b, m8, gpu.zeros((8, 8), G.MXFP8), dw) == "RT_ERR_DTYPE"
+    assert status(gpu.matmul_at_b, f(8, 40), gpu.zeros((8, 8), G.MXFP8), dw) == "RT_ERR_DTYPE"
+    assert status(gpu.matmul_at_b, m8, f(8, 8), gpu.zeros((40, 8), G.BF16)) == "RT_ERR_DTYPE"
+    assert status(gpu.matmul_at_b, m8, f(9, 8), dw) == "RT_ERR_SHAPE"
+    assert status(gpu.matmul_at_b, m8, f(8, 8), dw, f(9)) == "RT_ERR_SHAPE"
+    assert status(gpu.gemm, G.TN, m8, f(8, 8), dw, G.EPI_BIAS, f(8)) == "RT_ERR_INVALID"
+    assert status(gpu.linear_backward, m4, f(8, 8), f(40, 8), f(8, 40), dw) == "RT_ERR_DTYPE"
+    # masks
+    assert status(gpu.matmul_a_bt, f(8, 5), f(40, 5), f(8, 40), m4) == "RT_ERR_DTYPE"
+    assert status(gpu.matmul_a_bt, f(40, 5), f(8, 5), f(40, 8), m8) == "RT_ERR_SHAPE"
+    assert status(gpu.relu_bwd, m4, f(8, 40)) == "RT_ERR_DTYPE"
+    assert status(gpu.relu_bwd, m8, f(40, 8)) == "RT_ERR_SHAPE"
+    assert status(gpu.map_vjp, "relu", f(8, 40), m4, None, f(8, 40)) == "RT_ERR_DTYPE"
+    assert status(gpu.map_vjp, "relu", f(320), m8, None, f(8, 40)) == "RT_ERR_SHAPE"
+    assert status(gpu.map_vjp, "leaky_relu", f(8, 40), m8, None, f(8, 40)) == "RT_ERR_DTYPE"
+    # every other entry point
+    assert status(gpu.colsum, m8, f(40)) == "RT_ERR_DTYPE"
+    assert status(gpu.split_k, m8, m8, f(40, 40), f(40 * 40 * 2), 2, True) == "RT_ERR_DTYPE"
+    assert status(gpu.split_k_static, m8, m8, f(40, 40), 2, True) == "RT_ERR_DTYPE"
+    assert status(gpu.bias_add, m8, f(40)) == "RT_ERR_DTYPE"
+    assert status(gpu.relu, m8, m8) == "RT_ERR_SHAPE"
+    assert status(gpu.softmax_rows, m8, f(8, 40)) == "RT_ERR_DTYPE"
+    assert status(gpu.argmax_rows, m8, gpu.zeros((8,), G.U32)) == "RT_ERR_SHAPE"
+    assert status(gpu.map, "exp", m8, f(8, 40)) == "RT_ERR_DTYPE"
+    assert status(gpu.zip, "add", m8, m8, f(8, 40)) == "RT_ERR_DTYPE"
+    assert status(gpu.sgd, m8, m8, 0.1) == "RT_ERR_DTYPE"
+    assert status(gpu.reduce_to, m8, f(1, 40)) == "RT_ERR_DTYPE"
+    assert status(gpu.sum_all, m8, f()) == "RT_ERR_DTYPE"
+    with pytest.raises(ValueError):
+        gpu.upload(np.zeros(5, np.uint8), G.MXFP4, (8, 40))
+    gpu.sync()
+
+
+def test_wrap(gpu):
+    t = torch.arange(64, dtype=torch.float32, device="cuda")
+    torch.cuda.synchronize()
+    w = gpu.wrap(t.data_ptr(), (4, 16), owner=t)
+    assert np.array_equal(gpu.download(w).reshape(-1), np.arange(64, dtype=np.float32))
+    part = gpu.wrap(t.data_ptr() + 4 * 3, (5,))  # on an element's alignment only
+    assert np.array_equal(gpu.download(part), np.arange(3, 8, dtype=np.float32))
+    y = gpu.empty((4, 16))
+    gpu.map("scale", w, y, 2.0)
+    assert np.array_equal(gpu.download(y).reshape(-1), 2 * np.arange(64, dtype=np.float32))
+    gpu.map("scale", y, w, 2.0)
+    gpu.sync()
+    assert np.array_equal(t.cpu().numpy(), 4 * np.arange(64, dtype=np.float32))
+    w.free()
+    z = gpu.zeros((4, 16))  # the freed handle's memory is not the library's to reuse
+    gpu.sync()
+    assert np.array_equal(t.cpu().numpy(), 4 * np.arange(64, dtype=np.float32)) and not gpu.download(z).any()
+    host = np.zeros(64, np.float32)
+    assert status(gpu.wrap, 0, (4,)) == "RT_ERR_INVALID"
+    assert status(gpu.wrap, host.ctypes.data, (4,)) == "RT_ERR_INVALID"
+    assert status(gpu.wrap, t.data_ptr() + 2, (4,)) == "RT_ERR_INVALID"
+    assert status(gpu.wrap, t.data_ptr() + 4, (1, 1), G.MXFP4) == "RT_ERR_INVALID"
+    assert status(gpu.wrap, t.data_ptr(), (1 << 40,)) == "RT_ERR_SHAPE"
+    assert len(gpu.wrap(0, (0, 3))) == 0
+    other = G.Gpu(0)  # a context that still holds a wrapped tensor closes without it
+    other.wrap(t.data_ptr(), (64,))
+    other.close()
+    assert np.array_equal(t.cpu().numpy(), 4 * np.arange(64, dtype=np.float32))
+
+
+# ------------------------------------------------------------------ conversion
+SHAPES = [(1, 1), (1, 32), (1, 5000), (3, 33), (2, 31), (64, 128), (65, 129), (100, 1003), (130, 64), (300, 520)]
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("fmt", sorted(FMT))
+@pytest.mark.parametrize("dtype", sorted(DTYPE))
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_quantize_to_the_byte(gpu, rows, cols, dtype, fmt, transposed):
+    rng = np.random.default_rng(rows * 1000 + cols)
+    x = X.values(rng, rows, cols, spread=2.0)
+    if dtype == "f32":
+        x[0, :] *= np.float32(2.0 ** -140)  # subnormals
+        x[-1, -1] = 3e38
+    x64 = rounded(x, DTYPE[dtype])
+    t = gpu.upload(x64.T.copy() if transposed else x64, DTYPE[dtype])
+    q = gpu.upload(np.full(G.tensor_bytes((rows, cols), FMT[fmt]), 0xA5, np.uint8), FMT[fmt], (rows, cols))
+    gpu.convert_t(t, q) if transposed else gpu.convert(t, q)
+    code, byte, want = X.quantize(x64, FMT[fmt])
+    got, ref = gpu.download(q), X.pack(code, byte, FMT[fmt])
+    # the up to 255 bytes between codes and scales are not written
+    n = rows * (code.shape[1] // 2 if fmt == "fp4" else code.shape[1])
+    at = -(-n // 256) * 256
+    assert np.array_equal(got[at:], ref[at:])
+    assert np.array_equal(got[:n], ref[:n])
+    back = gpu.empty((rows, cols))
+    gpu.convert(q, back)
+    assert np.array_equal(gpu.download(back), want.astype(np.float32))
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("fmt", sorted(FMT))
+def test_quantize_ties_and_every_exponent(gpu, fmt, transposed):
+    # all bf16 values from 2^-133 up, positive and negative, each beside a maximum that puts it on every place of the grid
+    rng = np.random.default_rng(5)
+    bits = rng.integers(0, 0x7F80, size=(257, 96)).astype(np.uint16)
+    bits[:, 32:64] = (bits[:, 32:33] & 0x7F80) + rng.integers(0, 0x200, size=(257, 32)).astype(np.uint16)
+    bits[:, 32:64] = np.minimum(bits[:, 32:64], 0x7F7F)
+    bits[:, 64:] = np.minimum(0x3F80 + rng.integers(-0x300, 0x300, size=(257, 32)), 0x7F7F).astype(np.uint16)
+    bits |= (rng.integers(0, 2, size=bits.shape) << 15).astype(np.uint16)
+    x = G.bf16_bits_to_f32(bits).astype(np.float64)
+    q = gpu.zeros(x.shape, FMT[fmt])
+    gpu.convert_t(gpu.upload(bits.T.copy(), G.BF16), q) if transposed else gpu.convert(gpu.upload(bits, G.BF16), q)
+    code, byte, _ = X.quantize(x, FMT[fmt])
+    assert np.array_equal(gpu.download(q), X.pack(code, byte, FMT[fmt]))
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("fmt", sorted(FMT))
+@pytest.mark.parametrize("dtype", sorted(DTYPE))
+def test_quantize_not_finite(gpu, dtype, fmt, transposed):
+    x = X.values(np.random.default_rng(1), 70, 200)
+    x[3, 40], x[3, 100], x[64, 199], x[9, 0] = np.inf, -np.inf, np.nan, np.nan
+    x[5, 64:96] = np.inf
+    x64 = rounded(x, DTYPE[dtype])
+    t = gpu.upload(x64.T.copy() if transposed else x64, DTYPE[dtype])
+    q = gpu.zeros(x.shape, FMT[fmt])
+    gpu.convert_t(t, q) if transposed else gpu.convert(t, q)
+    want = X.quantize(x64, FMT[fmt])[2]
+    for out in (G.F32, G.BF16):
+        back = gpu.empty(x.shape, out)
+        gpu.convert(q, back)
+        assert np.array_equal(gpu.download_f32(back), want.astype(np.float32), equal_nan=True)
+
+
+@pytest.mark.parametrize("fmt", sorted(FMT))
+@pytest.mark.parametrize("dtype", sorted(DTYPE))
+@pytest.mark.parametrize("rows,cols", [(1, 7), (70, 256), (65, 1001)])
+def test_dequantize_any_bytes(gpu, rows, cols, dtype, fmt):
+    rng = np.random.default_rng(rows)
+    data = rng.integers(0, 256, size=G.tensor_bytes((rows, cols), FMT[fmt])).astype(np.uint8)
+    q = gpu.upload(data, FMT[fmt], (rows, cols))
+    want = G.mx_decode(data, (rows, cols), FMT[fmt])
+    out = gpu.empty((rows, cols), DTYPE[dtype])
+    gpu.convert(q, out)
+    with np.errstate(over="ignore"):
+        want = rounded(want, DTYPE[dtype])
+    got = gpu.download_f32(out)
+    assert np.array_equal(got, want.astype(np.float32), equal_nan=True)
+
+
+def test_empty_tensors(gpu):
+    for fmt in FMT.values():
+        for shape in ((0, 5), (5, 0), (0, 0)):
+            q = gpu.zeros(shape, fmt)
+            gpu.convert(gpu.zeros(shape), q)
+            gpu.convert_t(gpu.zeros(shape[::-1]), q)
+            gpu.convert(q, gpu.zeros(shape))
+            assert gpu.download(q).size == 0
+    gpu.sync()
+
+
+# ------------------------------------------------------------------ product
+def check_product(gpu, M, N, K, fa, out, epi, seed=0):
+    print(f"product {M}x{N} K {K} {fa}xfp4 -> {out} epilogue {epi}", flush=True)
+    rng = np.random.default_rng(seed + M * 7 + N * 3 + K)
+    a, av = mx_upload(gpu, X.values(rng, M, K), FMT[fa])
+    b, bv = mx_upload(gpu, X.values(rng, N, K, spread=0.3), G.MXFP4)
+    bias = rng.normal(size=(1, N)).astype(np.float32)
+    c = gpu.upload(np.full((M, N), 7.0, np.float32), DTYPE[out])
+    gpu.gemm(G.NT, a, b, c, epi, gpu.upload(bias) if epi else None)
+    want = av @ bv.T + (bias if epi else 0)
+    size = np.abs(av) @ np.abs(bv).T + np.abs(bias if epi else 0)
+    if epi == G.EPI_BIAS_RELU:
+        want = np.maximum(want, 0)
+    # K + 1 additions in f32, each off by at most one unit in the last place (2^-23) of what is summed so far, and
+    # for bf16 one rounding of the result
+    tol = (K + 8) * 2.0 ** -23 * size + (2.0 ** -8 * np.abs(want) if out == "bf16" else 0)
+    err = np.abs(gpu.download_f32(c).astype(np.float64) - want)
+    assert np.all(err <= tol), (err.max(), np.argwhere(err > tol)[:4])
+
+
+EPIS = [G.EPI_NONE, G.EPI_BIAS, G.EPI_BIAS_RELU]
+
+
+@pytest.mark.parametrize("fa", sorted(FMT))
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 10, 640), (5, 100, 129), (16, 16, 128), (17, 33, 4100), (37, 130, 1000),
+                                   (48, 64, 31), (64, 300, 2500), (65, 64, 128), (65, 10, 1), (130, 130, 1500),
+                                   (300, 257, 640), (256, 129, 384), (1500, 1003, 130), (1281, 1300, 200)])
+def test_product(gpu, M, N, K, fa):
+    for i, out in enumerate(("f32", "bf16")):
+        check_product(gpu, M, N, K, fa, out, EPIS[(M + N + K + i) % 3])
+
+
+@pytest.mark.parametrize("fa,M,N,K", [("fp4", 4100, 4090, 300), ("fp4", 4096, 4096, 1024), ("fp8", 4100, 4090, 300),
+                                      ("fp8", 4096, 4096, 700)])
+def test_product_large_tiles(gpu, fa, M, N, K):
+    check_product(gpu, M, N, K, fa, "f32", G.EPI_BIAS)
+    check_product(gpu, M, N, K, fa, "bf16", G.EPI_BIAS_RELU)
+
+
+@pytest.mark.parametrize("M", [3, 300])
+def test_product_of_8_bits_keeps_small_neighbours(gpu, M):
+    """Eight neighbouring products of very different sizes, the large ones cancelling: what is left are the small ones."""
+    x = np.zeros((M, 256))
+    x[:, 0::8], x[:, 1::8] = 448, -448
+    rng = np.random.default_rng(6)
+    for j in range(2, 8):
+        x[:, j::8] = np.ldexp(rng.integers(8, 16, size=(M, 32)) / 8.0, rng.integers(-9, 2, size=(M, 32)))
+    x = X.quantize(x, G.MXFP8)[2]
+    w = np.ones((70, 256))
+    w[:, 2:] = rng.choice([0.5, 1, 1.5, 3, 6], size=(70, 254))
+    w[:, 1::8] = w[:, 0::8]
+    a, av = mx_upload(gpu, x, G.MXFP8)
+    b, bv = mx_upload(gpu, w, G.MXFP4)
+    assert np.array_equal(av, x) and np.array_equal(bv, w)
+    c = gpu.empty((M, 70))
+    gpu.gemm(G.NT, a, b, c)
+    # every eight sums to a multiple of 2^-10, the small products of all 32 to below 6 · 4 · 6 · 32 < 2^13, where f32
+    # keeps 2^-11: 64 additions (two parts of each eight)
+    assert np.all(np.abs(gpu.download(c) - av @ bv.T) <= 64 * 2.0 ** -11)
+
+
+@pytest.mark.parametrize("M", [3, 200])
+def test_product_not_finite(gpu, M):
+    rng = np.random.default_rng(M)
+    x, w = X.values(rng, M, 200), X.values(rng, 90, 200)
+    x[1, 150] = np.nan
+    w[7, 3] = np.inf
+    for fa in FMT:
+        a, av = mx_upload(gpu, x, FMT[fa])
+        b, bv = mx_upload(gpu, w, G.MXFP4)
+        c = gpu.empty((M, 90))
+        gpu.gemm(G.NT, a, b, c)
+        nan = np.isnan(gpu.download(c))
+        assert nan[1].all() and nan[:, 7].all()
+        nan[1], nan[:, 7] = False, False
+        assert not nan.any()
+
+
+def test_product_without_columns(gpu):
+    for M in (3, 100):
+        a, b, c = gpu.zeros((M, 0), G.MXFP4), gpu.zeros((20, 0), G.MXFP4), gpu.upload(np.ones((M, 20), np.float32))
+        bias = np.arange(-10, 10, dtype=np.float32).reshape(1, 20)
+        gpu.gemm(G.NT, a, b, c, G.EPI_BIAS_RELU, gpu.upload(bias))
+        assert np.array_equal(gpu.download(c), np.maximum(np.repeat(bias, M, 0), 0))
+    gpu.gemm(G.NT, gpu.zeros((0, 9), G.MXFP4), gpu.zeros((20, 9), G.MXFP4), gpu.zeros((0, 20)))
+    gpu.sync()
+
+
+# ------------------------------------------------------------------ gradients from an 8-bit input
+def check_dw(gpu, rows, K, N, dtype, seed=0, x=None, d=None):
+    print(f"dW rows {rows} K {K} N {N} {dtype}", flush=True)
+    rng = np.random.default_rng(seed + rows + 5 * K + 11 * N)
+    x = np.maximum(X.values(rng, rows, K), 0) if x is None else x
+    d64 = rounded(rng.normal(size=(rows, N)) / 64 if d is None else d, DTYPE[dtype])
+    q, xv = mx_upload(gpu, x, G.MXFP8)
+    dw, db = gpu.upload(np.full((K, N), 7.0, np.float32)), gpu.upload(np.full((1, N), 7.0, np.float32))
+    gpu.matmul_at_b(q, gpu.upload(d64, DTYPE[dtype]), dw, colsum=db)
+    with np.errstate(invalid="ignore", over="ignore"):
+        want, size = xv.T @ d64, np.abs(xv).T @ np.abs(d64)
+        # every plane of every product is exact: three additions a row at most, and the planes of the slices
+        tol = (3 * rows + 40) * 2.0 ** -23 * size
+        got = gpu.download(dw).astype(np.float64)
+        fine = np.isfinite(size) & (size < 1e38)
+        assert np.array_equal(np.isnan(got[~fine]), np.isnan(want[~fine]))
+        err = np.abs(got - want)[fine]
+        assert np.all(err <= tol[fine]), err.max()
+        if fine.all():
+            err = np.abs(gpu.download(db)[0] - d64.sum(0))
+            assert np.all(err <= (rows + 8) * 2.0 ** -24 * np.abs(d64).sum(0))
+    return got, want
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPE))
+@pytest.mark.parametrize("rows,K,N", [(1, 1, 1), (1, 130, 10), (31, 100, 77), (37, 1024, 1000), (64, 128, 128),
+                                      (65, 129, 8), (300, 257, 300), (2048, 130, 7), (5000, 64, 250), (700, 1003, 777)])
+def test_dw(gpu, rows, K, N, dtype):
+    check_dw(gpu, rows, K, N, dtype)
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPE))
+def test_dw_many_tiles(gpu, dtype):
+    check_dw(gpu, 200, 4000, 2100, dtype)
+
+
+def test_dw_f32_range(gpu):
+    rng = np.random.default_rng(8)
+    d = (rng.normal(size=(200, 60)) * np.exp2(rng.integers(-100, 100, size=(1, 60)).astype(float))).astype(np.float32)
+    check_dw(gpu, 200, 70, 60, "f32", d=d)
+    # a gradient of infinities and NaN: its column alone
+    d = rng.normal(size=(200, 60)).astype(np.float32)
+    d[5, 3], d[6, 4], d[7, 5], d[8, 6] = np.inf, np.nan, -np.inf, 3.3e38
+    x = np.full((200, 70), 0.5, np.float32)
+    got, want = check_dw(gpu, 200, 70, 60, "f32", x=x, d=d)
+    assert np.all(got[:, 3] == np.inf) and np.isnan(got[:, 4]).all() and np.all(got[:, 5] == -np.inf)
+    assert np.allclose(got[:, 6], 1.65e38)
+    # a NaN in the saved input: its row of dW alone
+    x[9, 11] = np.nan
+    got, _ = check_dw(gpu, 200, 70, 60, "f32", x=x, d=rng.normal(size=(200, 60)))
+    assert np.isnan(got[11]).all() and np.isfinite(np.delete(got, 11, 0)).all()
+
+
+def test_dw_without_rows(gpu):
+    dw, db = gpu.upload(np.ones((20, 30), np.float32)), gpu.upload(np.ones((1, 30), np.float32))
+    gpu.matmul_at_b(gpu.zeros((0, 20), G.MXFP8), gpu.zeros((0, 30)), dw, colsum=db)
+    assert not gpu.download(dw).any() and not gpu.download(db).any()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 5), (37, 130), (200, 1003)])
+def test_masks_are_exact(gpu, rows, cols):
+    rng = np.random.default_rng(cols)
+    x = X.values(rng, rows, cols)
+    x[:, ::3] *= np.float32(1e-6)  # far below the step of their block
+    if rows > 1:
+        x[0] = -0.0
+    q = gpu.zeros((rows, cols), G.MXFP8)
+    gpu.convert(gpu.upload(x), q)
+    on = x > 0
+    g = rng.normal(size=(rows, cols)).astype(np.float32)
+    d = gpu.upload(g)
+    gpu.relu_bwd(q, d)
+    assert np.array_equal(gpu.download(d), np.where(on, g, 0))
+    dx = gpu.empty((rows, cols))
+    gpu.map_vjp("relu", gpu.upload(g), q, None, dx)
+    assert np.array_equal(gpu.download(dx), g * on)
+    # the mask of a product is that of the separate pass
+    for dtype, out in ((G.F32, G.F32), (G.BF16, G.BF16), (G.BF16, G.F32), (G.F16, G.F32)):
+        a, w = gpu.upload(rng.normal(size=(rows, 40)), dtype), gpu.upload(rng.normal(size=(cols, 40)), dtype)
+        plain, masked = gpu.empty((rows, cols), out), gpu.empty((rows, cols), out)
+        gpu.matmul_a_bt(a, w, plain)
+        gpu.matmul_a_bt(a, w, masked, relu_mask_from=q)
+        assert np.array_equal(gpu.download_f32(masked), np.where(on, gpu.download_f32(plain), 0))
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPE))
+def test_linear_backward_from_8_bits(gpu, dtype):
+    rows, K, N = 300, 200, 96
+    rng = np.random.default_rng(2)
+    x, d, w = X.values(rng, rows, K), rng.normal(size=(rows, N)), rng.normal(size=(K, N))
+    out = G.BF16 if dtype == "bf16" else G.F32
+    q, xv = mx_upload(gpu, x, G.MXFP8)
+    gd, gw = gpu.upload(d, DTYPE[dtype]), gpu.upload(w, DTYPE[dtype])
+    dx, dw, db = gpu.empty((rows, K), out), gpu.empty((K, N)), gpu.empty((1, N))
+    gpu.linear_backward(q, gd, gw, dx, dw, db)
+    dx2, dw2, db2 = gpu.empty((rows, K), out), gpu.empty((K, N)), gpu.empty((1, N))
+    gpu.matmul_at_b(q, gd, dw2, colsum=db2)
+    gpu.matmul_a_bt(gd, gw, dx2)
+    for one, two in ((dx, dx2), (dw, dw2), (db, db2)):
+        assert np.array_equal(gpu.download(one), gpu.download(two))
+    d64 = rounded(d, DTYPE[dtype])
+    assert np.all(np.abs(gpu.download(dw) - xv.T @ d64) <= (3 * rows + 40) * 2.0 ** -23 * (np.abs(xv).T @ np.abs(d64)))
+    gpu.linear_backward(q, gd, gw, None, dw2)
+    assert np.array_equal(gpu.download(dw), gpu.download(dw2))
+
+
+def test_a_quantized_layer_in_a_row(gpu):
+    """Weights laid out, activations converted, product, decoded: as a program chains them, twice, with other inputs."""
+    rng = np.random.default_rng(4)
+    w = rng.normal(size=(300, 200)).astype(np.float32) * 0.1
+    w4 = gpu.zeros((200, 300), G.MXFP4)
+    gpu.convert_t(gpu.upload(w), w4)
+    wv = X.quantize(w.T, G.MXFP4)[2]
+    bias = rng.normal(size=(1, 200)).astype(np.float32)
+    gb = gpu.upload(bias)
+    q, y = gpu.empty((100, 300), G.MXFP8), gpu.empty((100, 200))
+    for _ in range(2):
+        x = X.values(rng, 100, 300)
+        gpu.convert(gpu.upload(x), q)
+        gpu.gemm(G.NT, q, w4, y, G.EPI_BIAS_RELU, gb)
+        xv = X.quantize(x, G.MXFP8)[2]
+        tol = 308 * 2.0 ** -23 * (np.abs(xv) @ np.abs(wv).T + np.abs(bias))
+        assert np.all(np.abs(gpu.download(y) - np.maximum(xv @ wv.T + bias, 0)) <= tol)
