@@ -76,12 +76,19 @@ __device__ inline void dma16_asm(__amdgpu_buffer_rsrc_t rsrc, void* lds, int vof
                : "m0");
 }
 
-// The same with 4 bytes a lane: into LDS at lds + 4 * lane.
-__device__ inline void dma4_asm(__amdgpu_buffer_rsrc_t rsrc, void* lds, int voff, int soff) {
-  const int so = __builtin_amdgcn_readfirstlane(soff);
-  const unsigned dst = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) void*)lds);
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(dst), "v"(voff), "s"(rsrc), "s"(so)
-               : "m0");
+// dma16_asm to an LDS byte offset (lds_offset) instead of a pointer, whose
+// conversion would be checked for null at each use; and the same of 4 bytes a
+// lane, into LDS at dst + 4 * lane.
+__device__ inline unsigned lds_offset(void* lds) {
+  return (unsigned)(size_t)(__attribute__((address_space(3))) void*)lds;
+}
+__device__ inline void dma16_at(__amdgpu_buffer_rsrc_t rsrc, unsigned dst, int voff) {
+  const unsigned d = __builtin_amdgcn_readfirstlane(dst);
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(d), "v"(voff), "s"(rsrc) : "m0");
+}
+__device__ inline void dma4_at(__amdgpu_buffer_rsrc_t rsrc, unsigned dst, int voff) {
+  const unsigned d = __builtin_amdgcn_readfirstlane(dst);
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(d), "v"(voff), "s"(rsrc) : "m0");
 }
 #pragma clang diagnostic pop
 

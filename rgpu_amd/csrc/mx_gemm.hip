@@ -7,11 +7,14 @@
 // window that reaches 2^-13 below the power of two of the largest (measured: of
 // 2^16 - 2^16 + 2^s in one eight nothing below s = 3 comes back; between eights
 // and against the accumulator 2^-24).  4-bit products span 2^-2 to 36 and fit.
-// An 8-bit A does not (its values span 2^-9 to 448), so each of its fragments
-// goes in as two, the codes from 2 up and those below, zeros in the others'
-// places: a product then has its last bit at 2^-4 and its exponents within
-// 2^0 .. 2^10 or at 2^-10 and below 2^3, the eight sums are exact, and what is
-// left are f32 additions.
+// An 8-bit A does not (its values span 2^-9 to 448).  For an f32 C each of its
+// fragments therefore goes in as two, the codes from 2 up and those below, with
+// zeros in the others' places: products then reach from 2^-3 to below 2^12, or
+// from 2^-10 to below 2^4, the sums of eight are exact, and what is left are
+// f32 additions.  For a bf16 C it goes in whole (SPLIT false): what is dropped
+// is at most 2^-13 of a neighbouring product, whose 8-bit factor was itself
+// rounded by up to 2^-5 of it, and half the work is saved (8192 x 4096, K 4096:
+// 208 us split, 121 whole).
 //
 // What a lane holds.  Lane (g, r), g = lane / 16, r = lane % 16, of an operand
 // of 16 rows takes row r: the 4-bit codes of columns 32 g .. 32 g + 31 (16
@@ -85,8 +88,10 @@ struct Frag {
     for (int h = 0; h < BITS / 4; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const unsigned m = (v[h][i] >> 6) & 0x01010101u, mask = (m << 8) - m;  // 0xff where the bit is set
-        f.v[h][i] = v[h][i] & (large ? mask : ~mask);
+        // 0xff where the bit is set: selectors 8 to 11 spread bits 15 and 31 of
+        // the second and the first word over a byte.
+        const unsigned w = v[h][i], mask = __builtin_amdgcn_perm(w << 1, w << 9, 0x0b090a08u);
+        f.v[h][i] = w & (large ? mask : ~mask);
       }
     return f;
   }
@@ -94,7 +99,7 @@ struct Frag {
 
 // acc[u] += (B_u·Aᵀ of one step) for TN operands B; SA: which byte of A's scale
 // dword (B's: u % 4).
-template <int ABITS, int SA, int TN>
+template <int ABITS, bool SPLIT, int SA, int TN>
 __device__ inline void mfma_row(const Frag<ABITS>& a, const Frag<4> (&b)[TN], f4 (&acc)[TN], unsigned sa,
                                 const unsigned (&sb)[(TN + 3) / 4]) {
   auto one = [&](const Frag<ABITS>& x) {
@@ -104,7 +109,8 @@ __device__ inline void mfma_row(const Frag<ABITS>& a, const Frag<4> (&b)[TN], f4
                                                                 (int)sb[u / 4], SA, (int)sa);
     });
   };
-  if constexpr (ABITS == 8) {
+  if constexpr (SPLIT) {
+    static_assert(ABITS == 8, "4-bit products need no split");
     one(a.part(false));
     one(a.part(true));
   } else {
@@ -175,6 +181,7 @@ struct Side {
   int bytes;                  // the rows of a step that exist, from base
   int voff, row_step;
 
+  // The swizzle of a row, which repeats every 16 rows.
   __device__ static inline int sw(int row) { return BITS == 4 ? (row >> 2) & 3 : (row >> 1) & 7; }
   __device__ inline void init(const unsigned char* codes, int row_bytes, long long row0, long long rows, int wave,
                               int lane) {
@@ -184,25 +191,66 @@ struct Side {
     voff = row * row_bytes + 16 * ((lane % GR) ^ sw(row));
     row_step = RPI * WAVES * row_bytes;
   }
-  __device__ inline void issue(int step, unsigned char* lds, int wave) const {
+  __device__ inline void issue(int step, unsigned lds, int wave) const {
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<unsigned char*>(base + (long long)step * RB), (short)0, bytes, 0x00020000);
 #pragma unroll
     for (int i = 0; i < PER_WAVE; ++i)
-      rt_dev::dma16_asm(rsrc, lds + 1024 * (i * WAVES + wave), voff + i * row_step, 0);
+      rt_dev::dma16_at(rsrc, lds + 1024 * (i * WAVES + wave), voff + i * row_step);
   }
+  // row0: a multiple of 16, so that all fragments of a wave differ by constants.
   __device__ static inline Frag<BITS> frag(const unsigned char* lds, int row0, int g, int r) {
-    const int row = row0 + r;
     Frag<BITS> f;
 #pragma unroll
     for (int h = 0; h < BITS / 4; ++h)
-      f.v[h] = *reinterpret_cast<const u4*>(lds + row * RB + 16 * ((g + 4 * h) ^ sw(row)));
+      f.v[h] = *reinterpret_cast<const u4*>(lds + r * RB + 16 * ((g + 4 * h) ^ sw(r)) + row0 * RB);
     return f;
   }
 };
 
+// A wave tile's rows of C as T (f32, or bf16 bits), through the wave's own part
+// of LDS; N % 8 == 0 and C on 16 bytes.
+template <typename T, int TM, int TN>
+__device__ __forceinline__ void store_rows(const Args& p, const f4 (&acc)[TM][TN], const f4 (&bias)[TN],
+                                           unsigned char* smem, int wave, int lane, long long row0, int col0) {
+  constexpr int ROW = 16 * TN * sizeof(T), STRIDE = ROW + 16;      // bytes of a row of the tile
+  constexpr int LPR = ROW / 16, RPI = 64 / LPR;                    // lanes a row, rows an instruction
+  unsigned char* stage = smem + wave * 16 * STRIDE;
+  const int g = lane >> 4, r = lane & 15, rr = lane / LPR, cc = lane % LPR;
+  const int col = col0 + cc * (16 / (int)sizeof(T));
+  T* out = static_cast<T*>(p.c) + col;
+  static_for<0, TM>([&](auto tc) {
+    constexpr int t = decltype(tc)::value;
+#pragma unroll
+    for (int u = 0; u < TN; ++u) {
+      f4 v = acc[t][u];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = v[e] + bias[u][e];
+        if (p.relu) v[e] = fmaxf(v[e], 0.0f);
+      }
+      unsigned char* at = stage + r * STRIDE + (16 * u + 4 * g) * sizeof(T);
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f4*>(at) = v;
+      } else {
+        unsigned short h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = rt_mx::f32_to_bf16(v[e]);
+        *reinterpret_cast<u2*>(at) = u2{h[0] | ((unsigned)h[1] << 16), h[2] | ((unsigned)h[3] << 16)};
+      }
+    }
+    // The wave alone uses its part: its LDS operations are in order.
+#pragma unroll
+    for (int i = 0; i < 16 / RPI; ++i) {
+      const long long row = row0 + 16 * t + i * RPI + rr;
+      const u4 v = *reinterpret_cast<const u4*>(stage + (i * RPI + rr) * STRIDE + 16 * cc);
+      if (row < p.M && col < p.N) *reinterpret_cast<u4*>(out + row * p.N) = v;
+    }
+  });
+}
+
 // Block tile BM x BN, WGM x WGN waves, NS stages.
-template <int ABITS, int BM, int BN, int WGM, int WGN, int NS>
+template <int ABITS, bool SPLIT, int BM, int BN, int WGM, int WGN, int NS>
 __global__ __launch_bounds__(64 * WGM * WGN) void mx_gemm_kernel(Args p) {
   constexpr int WAVES = WGM * WGN, WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   using A = Side<ABITS, BM, WAVES>;
@@ -235,8 +283,9 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mx_gemm_kernel(Args p) {
   sa.init(p.a, p.a_row, m0, p.M, wave, lane);
   sb.init(p.b, p.b_row, n0, p.N, wave, lane);
 
+  const unsigned smem_at = rt_dev::lds_offset(smem);
   auto issue = [&](int step, int buf) {
-    unsigned char* lds = smem + buf * STAGE;
+    const unsigned lds = smem_at + buf * STAGE;
     sa.issue(step, lds, wave);
     sb.issue(step, lds + A::BYTES, wave);
 #pragma unroll
@@ -248,7 +297,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mx_gemm_kernel(Args p) {
       const unsigned char* src = (of_a ? p.a_scales : p.b_scales) + 256 * ((long long)step * total + min(at, total - 1));
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<unsigned char*>(src), (short)0, at < total ? 256 : 0, 0x00020000);
-      rt_dev::dma4_asm(rsrc, lds + A::BYTES + B::BYTES + 256 * grp, 4 * lane, 0);
+      rt_dev::dma4_at(rsrc, lds + A::BYTES + B::BYTES + 256 * grp, 4 * lane);
     }
   };
 
@@ -280,7 +329,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mx_gemm_kernel(Args p) {
   auto mfmas = [&](const Set& s) {
     static_for<0, TM>([&](auto tc) {
       constexpr int t = decltype(tc)::value;
-      mfma_row<ABITS, t & 3, TN>(s.a[t], s.b, acc[t], s.as[t / 4], s.bs);
+      mfma_row<ABITS, SPLIT, t & 3, TN>(s.a[t], s.b, acc[t], s.as[t / 4], s.bs);
     });
   };
 
@@ -317,6 +366,16 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mx_gemm_kernel(Args p) {
   f4 bias[TN];
 #pragma unroll
   for (int u = 0; u < TN; ++u) bias[u] = load_bias(p, (int)n0 + wn + 16 * u + 4 * g);
+  // Whole rows: 16 rows of the wave's columns at a time go through LDS, so that
+  // a store instruction covers a row's 64 to 256 bytes (a lane's own 8 or 16
+  // are 32 or 64 consecutive ones for four lanes).
+  const bool whole = p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
+  if (whole) {
+    __syncthreads();  // no wave reads its fragments any more
+    if (p.out_bf16) store_rows<unsigned short, TM, TN>(p, acc, bias, smem, wave, lane, m0 + wm, (int)n0 + wn);
+    else store_rows<float, TM, TN>(p, acc, bias, smem, wave, lane, m0 + wm, (int)n0 + wn);
+    return;
+  }
   static_for<0, TM>([&](auto tc) {
     static_for<0, TN>([&](auto uc) {
       constexpr int t = decltype(tc)::value, u = decltype(uc)::value;
@@ -371,7 +430,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void mx_rows_kernel(Args p) {
       if (k0 + i < p.steps) {
         static_for<0, TM>([&](auto tc) {
           constexpr int t = decltype(tc)::value;
-          mfma_row<ABITS, t & 3, 1>(fa[i][t], fb[i], acc[t], sa[i], sb[i]);
+          mfma_row<ABITS, ABITS == 8, t & 3, 1>(fa[i][t], fb[i], acc[t], sa[i], sb[i]);
         });
       }
     }
@@ -388,13 +447,26 @@ __global__ __launch_bounds__(64 * kRowWaves) void mx_rows_kernel(Args p) {
   }
 }
 
-template <int ABITS, int BM, int BN, int WGM, int WGN, int NS>
+template <int ABITS, bool SPLIT, int BM, int BN, int WGM, int WGN, int NS>
 hipError_t launch_tiles(hipStream_t s, Args p) {
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
-  rt::launch(mx_gemm_kernel<ABITS, BM, BN, WGM, WGN, NS>, dim3((unsigned)((long long)p.tiles_m * p.tiles_n)),
-             dim3(64 * WGM * WGN), 0, s, p);
+  rt::launch(mx_gemm_kernel<ABITS, SPLIT, BM, BN, WGM, WGN, NS>,
+             dim3((unsigned)((long long)p.tiles_m * p.tiles_n)), dim3(64 * WGM * WGN), 0, s, p);
   return hipGetLastError();
+}
+
+// A product of more rows.
+template <int ABITS, bool SPLIT>
+hipError_t launch_many(hipStream_t s, const Args& p) {
+  auto tiles = [&](int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+  if constexpr (ABITS == 4) {
+    if (tiles(256, 256) >= 256) return launch_tiles<4, false, 256, 256, 2, 4, 4>(s, p);
+  } else {
+    if (tiles(256, 128) >= 256) return launch_tiles<8, SPLIT, 256, 128, 4, 2, 3>(s, p);
+  }
+  if (tiles(128, 128) >= 128) return launch_tiles<ABITS, SPLIT, 128, 128, 2, 2, 3>(s, p);
+  return launch_tiles<ABITS, SPLIT, 64, 64, 2, 2, 4>(s, p);
 }
 
 template <int ABITS>
@@ -408,14 +480,10 @@ hipError_t launch(hipStream_t s, const Args& p) {
     else rt::launch(mx_rows_kernel<ABITS, 4>, grid, block, 0, s, p);
     return hipGetLastError();
   }
-  auto tiles = [&](int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-  if constexpr (ABITS == 4) {
-    if (tiles(256, 256) >= 256) return launch_tiles<4, 256, 256, 2, 4, 4>(s, p);
-  } else {
-    if (tiles(256, 128) >= 256) return launch_tiles<8, 256, 128, 4, 2, 3>(s, p);
+  if constexpr (ABITS == 8) {
+    if (!p.out_bf16) return launch_many<8, true>(s, p);
   }
-  if (tiles(128, 128) >= 128) return launch_tiles<ABITS, 128, 128, 2, 2, 4>(s, p);
-  return launch_tiles<ABITS, 64, 64, 2, 2, 4>(s, p);
+  return launch_many<ABITS, false>(s, p);
 }
 
 }  // namespace
