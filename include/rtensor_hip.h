@@ -62,7 +62,8 @@ typedef enum {
  *   - from the next multiple of 256 bytes on, the scale bytes (e + 127; 255 makes
  *     the block NaN), in the order in which the matrix units take them: for each
  *     128 columns, for each 64 rows (the last may be short), 256 bytes of which
- *     byte 4·(16·g + r) + t is that of row 16·t + r and columns 32·g .. 32·g+31.
+ *     byte 4·(16·g + r) + t is that of row 16·t + r and columns 32·g .. 32·g+31;
+ *     0 where there is no such row or column.
  * rt_tensor_bytes gives the size; transfers move the bytes as they are. */
 typedef enum { RT_F32 = 0, RT_BF16 = 1, RT_F16 = 2, RT_U32 = 3, RT_MXFP4 = 4, RT_MXFP8 = 5 } rt_dtype;
 

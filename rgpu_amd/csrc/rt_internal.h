@@ -299,11 +299,12 @@ hipError_t mx_relu_vjp_launch(hipStream_t s, const MxTensor& mask, const float* 
 // C [M, N] = A·Bᵀ with A [M, K] and B RT_MXFP4 [N, K]; epi none, bias or bias and ReLU.
 hipError_t mx_gemm_launch(hipStream_t s, const MxTensor& a, const MxTensor& b, void* C, int out_dtype, int epi,
                           const float* bias);
-// C [K, N] (f32) = Xᵀ·δ with X RT_MXFP8 [rows, K] and δ [rows, N]; scratch holds
+// C [K, N] (f32) = Xᵀ·δ with X RT_MXFP8 [rows, K] and δ [rows, N], rows, K and N
+// above 0, and δ's column sums into colsum if given; scratch holds
 // mx_dw_scratch_elems floats.
-size_t mx_dw_scratch_elems(const MxTensor& x, int delta_dtype, long long N);
+size_t mx_dw_scratch_elems(const MxTensor& x, const void* delta, int delta_dtype, long long N, bool colsum);
 hipError_t mx_dw_launch(hipStream_t s, const MxTensor& x, const void* delta, int delta_dtype, long long N, float* C,
-                        float* scratch);
+                        float* colsum, float* scratch, size_t scratch_elems);
 
 // ---------------------------------------------------------------- optimizer
 struct OptTensor {

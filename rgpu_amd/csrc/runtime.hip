@@ -555,22 +555,18 @@ static int mx_gemm(rt_ctx* c, rt_layout layout, const rt_buf* a, const rt_buf* b
   if (epi != RT_EPI_NONE) return fail(c, RT_ERR_INVALID, "the TN product of an 8-bit A has no epilogue");
   if (colsum && (colsum->dtype != RT_F32 || colsum->n != N)) return fail(c, RT_ERR_SHAPE, "colsum must be f32 [%zu]", N);
   if (N == 0) return RT_OK;
+  if (M == 0 || K == 0) {  // no input column: the bias gradient alone; no row: zeros
+    if (M > 0)
+      HIP_TRY(c, fill_i32_launch(c->stream, static_cast<int*>(out->ptr), 0, M * N), "gradient of no rows");
+    return colsum ? rt_colsum(c, b, colsum) : RT_OK;
+  }
   const MxTensor x = mx_tensor(a);
-  if ((rc = ensure_scratch(c, std::max(mx_dw_scratch_elems(x, b->dtype, (long long)N),
-                                       colsum ? colsum_scratch_elems((int)K, (int)N, b->dtype) : 0))))
-    return rc;
-  if (M > 0) {
-    Launch L(c, "mx_gemm_tn");
-    HIP_TRY(c, mx_dw_launch(c->stream, x, b->ptr, b->dtype, (long long)N, static_cast<float*>(out->ptr), c->scratch),
-            "gradient from an 8-bit input");
-  }
-  if (colsum) {
-    Launch L(c, "colsum");
-    HIP_TRY(c,
-            colsum_launch(c->stream, b->ptr, b->dtype, (int)K, (int)N, static_cast<float*>(colsum->ptr), c->scratch,
-                          c->scratch_elems),
-            "colsum");
-  }
+  if ((rc = ensure_scratch(c, mx_dw_scratch_elems(x, b->ptr, b->dtype, (long long)N, colsum != nullptr)))) return rc;
+  Launch L(c, "mx_gemm_tn");
+  HIP_TRY(c,
+          mx_dw_launch(c->stream, x, b->ptr, b->dtype, (long long)N, static_cast<float*>(out->ptr),
+                       colsum ? static_cast<float*>(colsum->ptr) : nullptr, c->scratch, c->scratch_elems),
+          "gradient from an 8-bit input");
   return RT_OK;
 }
 

@@ -356,8 +356,38 @@ def test_dw(gpu, rows, K, N, dtype):
 
 
 @pytest.mark.parametrize("dtype", sorted(DTYPE))
-def test_dw_many_tiles(gpu, dtype):
-    check_dw(gpu, 200, 4000, 2100, dtype)
+@pytest.mark.parametrize("rows,K,N", [(200, 4000, 2100), (200, 4000, 2104), (70, 4100, 4096), (9000, 256, 512),
+                                      (20001, 300, 264), (5000, 520, 8)])
+def test_dw_many_tiles_or_slices(gpu, rows, K, N, dtype):
+    check_dw(gpu, rows, K, N, dtype)
+
+
+@pytest.mark.parametrize("N", [300, 304])
+@pytest.mark.parametrize("rows", [77, 9000])
+def test_dw_f16_scales_beyond_f16(gpu, rows, N):
+    # blocks that f16 cannot hold (too large, or with bits below 2^-24) beside some that it can
+    rng = np.random.default_rng(N)
+    x = rng.normal(size=(rows, 300)).astype(np.float32)
+    x[:, 64:96] *= np.float32(2.0 ** 18)
+    x[: rows // 2, 128:160] *= np.float32(2.0 ** -30)
+    check_dw(gpu, rows, 300, N, "f16", x=x)
+    x[:, 64:96], x[:, 128:160] = 65504.0, 2.0 ** -24  # the largest and the smallest of f16
+    check_dw(gpu, rows, 300, N, "f16", x=x)
+
+
+def test_dw_absent_rows_have_no_scale(gpu):
+    rows, K, N = 70, 200, 64
+    rng = np.random.default_rng(3)
+    x, d = np.maximum(rng.normal(size=(rows, K)), 0), rng.normal(size=(rows, N))
+    code, byte, xv = X.quantize(x, G.MXFP8)
+    data = X.pack(np.concatenate([code, np.zeros((58, 256), np.uint8)]),
+                  np.concatenate([byte, np.full((58, 8), 255, np.uint8)]), G.MXFP8)
+    at, full = -(-rows * 256 // 256) * 256, 128 * 256
+    q = gpu.upload(np.concatenate([data[:at], data[full:]]), G.MXFP8, (rows, K))
+    for dtype in DTYPE.values():
+        dw, d64 = gpu.empty((K, N)), rounded(d, dtype)
+        gpu.matmul_at_b(q, gpu.upload(d64, dtype), dw)
+        assert np.all(np.abs(gpu.download(dw) - xv.T @ d64) <= (3 * rows + 40) * 2.0 ** -23 * (np.abs(xv).T @ np.abs(d64)))
 
 
 def test_dw_f32_range(gpu):
@@ -416,7 +446,8 @@ def test_linear_backward_from_8_bits(gpu, dtype):
     x, d, w = X.values(rng, rows, K), rng.normal(size=(rows, N)), rng.normal(size=(K, N))
     out = G.BF16 if dtype == "bf16" else G.F32
     q, xv = mx_upload(gpu, x, G.MXFP8)
-    gd, gw = gpu.upload(d, DTYPE[dtype]), gpu.upload(w, DTYPE[dtype])
+    d64 = rounded(d, DTYPE[dtype])
+    gd, gw = gpu.upload(d64, DTYPE[dtype]), gpu.upload(w, DTYPE[dtype])
     dx, dw, db = gpu.empty((rows, K), out), gpu.empty((K, N)), gpu.empty((1, N))
     gpu.linear_backward(q, gd, gw, dx, dw, db)
     dx2, dw2, db2 = gpu.empty((rows, K), out), gpu.empty((K, N)), gpu.empty((1, N))
@@ -424,7 +455,6 @@ def test_linear_backward_from_8_bits(gpu, dtype):
     gpu.matmul_a_bt(gd, gw, dx2)
     for one, two in ((dx, dx2), (dw, dw2), (db, db2)):
         assert np.array_equal(gpu.download(one), gpu.download(two))
-    d64 = rounded(d, DTYPE[dtype])
     assert np.all(np.abs(gpu.download(dw) - xv.T @ d64) <= (3 * rows + 40) * 2.0 ** -23 * (np.abs(xv).T @ np.abs(d64)))
     gpu.linear_backward(q, gd, gw, None, dw2)
     assert np.array_equal(gpu.download(dw), gpu.download(dw2))
