@@ -6,8 +6,9 @@
 // without rounding, and an f16 too where its block's scale is from 2^-15 to 2^7.
 // bf16 δ is multiplied as it stands; f16 δ as well where the block's part of X
 // has only such scales (a block looks its scales over first: 1/32 of its codes'
-// bytes), else as two bf16 planes (11 bits); f32 δ as three (24 bits, each plane
-// the next eight by truncation).  So every product is exact, and the sums are
+// bytes; 262144 rows of 512 x 512 160 us, 408 in planes), else as two bf16
+// planes (11 bits); f32 δ as three (24 bits, each plane the next eight by
+// truncation).  So every product is exact, and the sums are
 // f32.  The scale of X varies along the rows that are summed, so it cannot stay
 // outside the product: X is decoded on its way into LDS, where a thread holds 16
 // columns of one row, which share a scale.
@@ -44,8 +45,9 @@ struct Args {
   const unsigned char* x_scales;
   const void* delta;
   float* c;
-  float* shares;   // column sums of δ, [slices, tiles_m, N]: of a slice's 64-row pieces tile row t adds those with
-                   // index % tiles_m == t (blocks of both bodies share a slice); or null
+  float* shares;   // column sums of δ, [slices, sharers, N]: of a slice's 64-row pieces tile row t < sharers adds those
+                   // with index % sharers == t (blocks of both bodies share a slice); or null
+  int sharers;
   long long rows;  // summed
   int K, N;        // of C
   int x_row;       // bytes of a row of codes
@@ -84,21 +86,6 @@ __device__ inline u2 lds_tr(const unsigned short* p) {
   return __builtin_bit_cast(u2, r);
 }
 
-// 16 consecutive codes of one row of X and their scale byte.
-struct XChunk {
-  u4 w;
-  unsigned char byte;
-  __device__ inline void load(const Args& p, long long row, long long re, int col) {
-    w = u4{0u, 0u, 0u, 0u};
-    byte = 0;
-    if (row < re && col < p.x_row) {
-      w = *reinterpret_cast<const u4*>(p.x + row * p.x_row + col);
-      byte = p.x_scales[((long long)(col / 128) * p.x_groups + row / 64) * 256 + 4 * (16 * (col % 128 / 32) + row % 16) +
-                        row % 64 / 16];
-    }
-  }
-};
-
 // 16 codes as 16 bf16 or f16.
 template <bool F16>
 __device__ inline void decode16(const u4& w, unsigned byte, u4 (&out)[2]) {
@@ -122,6 +109,54 @@ __device__ inline void decode16(const u4& w, unsigned byte, u4 (&out)[2]) {
 __device__ inline __amdgpu_buffer_rsrc_t bounded_rsrc(const void* base, long long bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0,
                                            (int)max(0LL, min(bytes, 0x7ffffff0LL)), 0x00020000);
+}
+
+// X of a stage: a thread's chunks of 16 codes are 32 rows apart, in the same
+// columns; the dword that holds the scale of one holds those of all (of the
+// 64-row group).  Rows past the slice's end are zeros; columns past X's last come
+// from elsewhere, in rows of C that are not stored.
+template <int ROWS, int BM, int THREADS>
+struct XSide {
+  static constexpr int XR = BM / 16, CHUNKS = ROWS * XR / THREADS;
+  static_assert(THREADS / XR == 32 && CHUNKS * 32 == ROWS, "chunks 32 rows apart");
+  struct Raw {
+    u4 w[CHUNKS];
+    unsigned scales;
+  };
+  int k, voff, svoff;  // row and column of the first chunk
+  __device__ inline void init(const Args& p, const Place& at, int tid) {
+    const int c = at.m0 % 128 / 16 + tid % XR;  // chunk of its 128 columns, and beyond
+    k = tid / XR;
+    voff = k * p.x_row + 16 * (tid % XR);
+    svoff = c / 8 * (p.x_groups * 256) + 4 * (16 * (c % 8 / 2) + k % 16);
+  }
+  __device__ inline void load(const Args& p, const Place& at, int s, Raw& x) const {
+    const long long row = at.rb + (long long)s * ROWS, group = row / 64;
+    const long long first = (long long)(at.m0 / 128) * p.x_groups + group, all = (long long)(p.x_row / 128) * p.x_groups;
+    const __amdgpu_buffer_rsrc_t rsrc = bounded_rsrc(p.x + row * p.x_row + at.m0, (at.re - row) * p.x_row - at.m0);
+    const __amdgpu_buffer_rsrc_t srsrc = bounded_rsrc(p.x_scales + first * 256, (all - first) * 256);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) x.w[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, voff + i * 32 * p.x_row, 0, 0);
+    x.scales = __builtin_amdgcn_raw_buffer_load_b32(srsrc, svoff, 0, 0);
+  }
+  // Chunk i as 16 halves.  Absent rows have no scale either (their byte may be any).
+  template <bool F16>
+  __device__ inline void decode(const Place& at, int s, const Raw& x, int i, u4 (&h)[2]) const {
+    const long long row = at.rb + (long long)s * ROWS + k + 32 * i;
+    const unsigned byte = (x.scales >> (8 * ((int)row % 64 / 16))) & 0xffu;
+    decode16<F16>(x.w[i], row < at.re ? byte : 0u, h);
+  }
+};
+
+// acc += of 32 rows; the operands swapped (D = δᵀ·X), so that lane (g, r) ends
+// with row r and four consecutive columns.
+template <bool F16>
+__device__ inline f4 mfma(const u4& a, const u4& b, const f4& acc) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b), __builtin_bit_cast(f16x8, a), acc, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), acc, 0, 0,
+                                                   0);
 }
 
 // C's tile (or its plane of the slice): lane (g, r) holds four consecutive
@@ -158,7 +193,7 @@ __device__ __forceinline__ void store_shares(const Args& p, const float (&cs)[8]
 #pragma unroll
   for (int e = 0; e < 8; ++e) red[(tid / CH) * CH * 8 + 8 * (tid % CH) + e] = cs[e];
   __syncthreads();
-  float* out = p.shares + ((long long)at.slice * p.tiles_m + at.tile_m) * p.N;
+  float* out = p.shares + ((long long)at.slice * p.sharers + at.tile_m) * p.N;
   for (int col = tid; col < CH * 8 && at.n0 + col < p.N; col += THREADS) {
     float v = 0.0f;
     for (int j = 0; j < THREADS / CH; ++j) v += red[j * CH * 8 + col];
@@ -166,7 +201,7 @@ __device__ __forceinline__ void store_shares(const Args& p, const float (&cs)[8]
   }
 }
 
-// ---------------------------------------------------------------- δ in bf16 planes
+// ---------------------------------------------------------------- through registers
 // The upper halves of two words, lo first.
 __device__ inline unsigned pack_hi(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 
@@ -188,49 +223,90 @@ __device__ inline void split8(const float (&v)[8], u4 (&out)[P]) {
   }
 }
 
-// Eight consecutive values of δ: planes P, and rows of a stage (two bf16 k-steps
-// of 32 where there is one plane, so that a stage has the same work).
-template <int DT>
-struct Delta;
-template <>
-struct Delta<RT_BF16> {
-  static constexpr int PLANES = 1, ROWS = 64;
-  using T = unsigned short;
-  static __device__ inline float get(T v) { return __uint_as_float((unsigned)v << 16); }
+// What δ is and how it is multiplied: its planes, the rows of a stage (two MFMA
+// k-steps of 32 where there is one plane, one else), and a chunk of eight values.
+// Halves come as five dwords from the one that holds the first value on, shifted
+// to it, so that rows may start on any of them.
+enum Kind { kBf16, kF16, kF16Planes, kF32 };
+template <int KIND>
+struct Delta {
+  static constexpr bool F16 = KIND == kF16;
+  static constexpr int PLANES = KIND == kF16Planes ? 2 : 1, ROWS = PLANES == 1 ? 64 : 32, SIZE = 2;
+  struct Raw {
+    u4 w;
+    unsigned last;
+  };
+  static __device__ inline Raw load(__amdgpu_buffer_rsrc_t rsrc, unsigned at) {
+    const int a = (int)(at & ~3u);
+    return Raw{__builtin_amdgcn_raw_buffer_load_b128(rsrc, a, 0, 0),
+               (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rsrc, a + 16, 0, 0)};
+  }
+  static __device__ inline u4 halves(const Raw& x, unsigned at) {
+    const unsigned sh = 8 * (at & 3u);
+    u4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_alignbit(i < 3 ? x.w[i + 1] : x.last, x.w[i], sh);
+    return v;
+  }
+  static __device__ inline void values(const Raw& x, unsigned at, float (&v)[8]) {
+    const u4 h = halves(x, at);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned short b = (unsigned short)(h[e / 2] >> (16 * (e % 2)));
+      if constexpr (KIND == kBf16) v[e] = __uint_as_float((unsigned)b << 16);
+      else v[e] = (float)__builtin_bit_cast(_Float16, b);
+    }
+  }
+  static __device__ inline void planes(const Raw& x, unsigned at, u4 (&out)[PLANES]) {
+    if constexpr (PLANES == 1) {
+      out[0] = halves(x, at);
+    } else {
+      float v[8];
+      values(x, at, v);
+      split8<PLANES>(v, out);
+    }
+  }
 };
 template <>
-struct Delta<RT_F16> {
-  static constexpr int PLANES = 2, ROWS = 32;
-  using T = _Float16;
-  static __device__ inline float get(T v) { return (float)v; }
-};
-template <>
-struct Delta<RT_F32> {
-  static constexpr int PLANES = 3, ROWS = 32;
-  using T = float;
-  static __device__ inline float get(T v) { return v; }
+struct Delta<kF32> {
+  static constexpr bool F16 = false;
+  static constexpr int PLANES = 3, ROWS = 32, SIZE = 4;
+  struct Raw {
+    u4 w[2];
+  };
+  static __device__ inline Raw load(__amdgpu_buffer_rsrc_t rsrc, unsigned at) {
+    return Raw{{__builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)at, 0, 0),
+                __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)at + 16, 0, 0)}};
+  }
+  static __device__ inline void values(const Raw& x, unsigned, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(x.w[e / 4][e % 4]);
+  }
+  static __device__ inline void planes(const Raw& x, unsigned at, u4 (&out)[3]) {
+    float v[8];
+    values(x, at, v);
+    split8<3>(v, out);
+  }
 };
 
-// LDS of the planes' two stages: [row][BM + 16] of X, then [row][BN + 16] of
-// each plane, in halves.
-template <int DT, int BM, int BN>
-constexpr int planes_lds() {
-  return 2 * Delta<DT>::ROWS * (BM + 16 + Delta<DT>::PLANES * (BN + 16));
+// LDS of two stages: [row][BM + 16] of X, then [row][BN + 16] of each plane, in halves.
+template <int KIND, int BM, int BN>
+constexpr int staged_lds() {
+  return 2 * Delta<KIND>::ROWS * (BM + 16 + Delta<KIND>::PLANES * (BN + 16));
 }
 
 // Any δ, any alignment: both operands through registers, where X is decoded and
-// δ split, into the LDS stage that the MFMAs of the other one do not read.
-template <int DT, int BM, int BN, int WGM, int WGN>
-__device__ __forceinline__ void planes_body(const Args& p, const Place& at, unsigned short* smem) {
-  using D = Delta<DT>;
-  using T = typename D::T;
+// δ split, into the LDS stage that the MFMAs of the other one do not read.  Loads
+// go out two stages ahead of that, three ahead of their MFMAs.
+template <int KIND, int BM, int BN, int WGM, int WGN>
+__device__ __forceinline__ void staged_body(const Args& p, const Place& at, unsigned short* smem) {
+  using D = Delta<KIND>;
   constexpr int THREADS = 64 * WGM * WGN, ROWS = D::ROWS, P = D::PLANES;
   constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   constexpr int SA = BM + 16, SB = BN + 16, STAGE = ROWS * (SA + P * SB);
-  constexpr int XC = ROWS * BM / 16 / THREADS, DC = ROWS * BN / 8 / THREADS;  // chunks a thread
-  constexpr int CH = BN / 8;
-  static_assert(XC * THREADS * 16 == ROWS * BM && DC * THREADS * 8 == ROWS * BN, "chunks split evenly");
-  static_assert(THREADS % CH == 0, "a thread's chunks of δ are all of the same columns");
+  constexpr int CH = BN / 8, KR = THREADS / CH, DC = ROWS / KR;  // chunks a row of δ, rows between a thread's, chunks
+  using X = XSide<ROWS, BM, THREADS>;
+  static_assert(THREADS % CH == 0 && DC * KR == ROWS, "a thread's chunks of δ are all of the same columns");
   static_assert(THREADS * 8 * 4 <= 2 * STAGE * 2, "column sums fit in LDS");
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -238,58 +314,68 @@ __device__ __forceinline__ void planes_body(const Args& p, const Place& at, unsi
   const int wm = (wave / WGN) * WM, wn = (wave % WGN) * WN;
   const int stages = (int)((at.re - at.rb + ROWS - 1) / ROWS);  // at least one, by the host's plan
 
-  XChunk x[XC];
-  T d[DC][8];
-  const T* delta = static_cast<const T*>(p.delta);
-  const int dcol = at.n0 + 8 * (tid % CH);
-  auto load = [&](int s) {
-    const long long base = at.rb + (long long)s * ROWS;
-#pragma unroll
-    for (int i = 0; i < XC; ++i) {
-      const int idx = tid + THREADS * i;
-      x[i].load(p, base + idx / (BM / 16), at.re, at.m0 + 16 * (idx % (BM / 16)));
-    }
-#pragma unroll
-    for (int i = 0; i < DC; ++i) {
-      const long long row = base + (tid + THREADS * i) / CH;
-      const T* src = delta + row * p.N + dcol;
-      if (row < at.re && dcol + 8 <= p.N) {
-        __builtin_memcpy(d[i], src, sizeof d[i]);  // whatever the alignment
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[i][e] = row < at.re && dcol + e < p.N ? src[e] : T(0);
-      }
-    }
+  X xs;
+  xs.init(p, at, tid);
+  // δ is addressed from the dword that holds its slice's first value of the
+  // stage, to the one that holds its last; columns past N are the next row's.
+  const unsigned dvoff = (unsigned)D::SIZE * ((unsigned)(tid / CH) * p.N + 8 * (tid % CH)), dstep = D::SIZE * KR * p.N;
+  auto delta_at = [&](int s) {  // address of the stage's first value
+    return reinterpret_cast<uintptr_t>(p.delta) +
+           (unsigned long long)D::SIZE * ((at.rb + (long long)s * ROWS) * p.N + at.n0);
   };
-  const bool do_cs = p.shares != nullptr;
+  struct Raw {
+    typename X::Raw x;
+    typename D::Raw d[DC];
+  };
+  auto load = [&](int s, Raw& raw) {
+    xs.load(p, at, s, raw.x);
+    const uintptr_t from = delta_at(s), base = from & ~(uintptr_t)3;
+    const long long rows = at.re - at.rb - (long long)s * ROWS;
+    const long long bytes = rows > 0 ? (D::SIZE * (rows * p.N - at.n0) + (long long)(from - base) + 3) & ~3LL : 0;
+    const __amdgpu_buffer_rsrc_t rsrc = bounded_rsrc(reinterpret_cast<const void*>(base), bytes);
+#pragma unroll
+    for (int i = 0; i < DC; ++i) raw.d[i] = D::load(rsrc, (unsigned)(from - base) + dvoff + i * dstep);
+  };
+  const bool do_cs = p.shares != nullptr && at.tile_m < p.sharers;
   float cs[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  auto store = [&](int s) {
+  auto store = [&](int s, const Raw& raw) {
     unsigned short* a = smem + (s & 1) * STAGE;
     unsigned short* b = a + ROWS * SA;
 #pragma unroll
-    for (int i = 0; i < XC; ++i) {
-      const int idx = tid + THREADS * i;
+    for (int i = 0; i < X::CHUNKS; ++i) {
       u4 h[2];
-      decode16<false>(x[i].w, x[i].byte, h);
-      u4* to = reinterpret_cast<u4*>(a + (idx / (BM / 16)) * SA + 16 * (idx % (BM / 16)));
+      xs.template decode<D::F16>(at, s, raw.x, i, h);
+      u4* to = reinterpret_cast<u4*>(a + (xs.k + 32 * i) * SA + 16 * (tid % X::XR));
       to[0] = h[0];
       to[1] = h[1];
     }
-    const bool add = do_cs && s * ROWS / 64 % p.tiles_m == at.tile_m;
+    const unsigned off = (unsigned)(delta_at(s) & 3);
+    // Half of the last dword may be a value of an absent row.
+    auto chunk = [&](int i) {
+      typename D::Raw d = raw.d[i];
+      if constexpr (D::SIZE == 2) {
+        const bool in = at.rb + (long long)s * ROWS + tid / CH + KR * i < at.re;
+        d.w = in ? d.w : u4{0u, 0u, 0u, 0u};
+        d.last = in ? d.last : 0u;
+      }
+      return d;
+    };
 #pragma unroll
     for (int i = 0; i < DC; ++i) {
-      float v[8];
+      u4 h[P];
+      D::planes(chunk(i), off + dvoff + i * dstep, h);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = D::get(d[i][e]);
-      if (add) {
+      for (int q = 0; q < P; ++q)
+        *reinterpret_cast<u4*>(b + q * ROWS * SB + (tid / CH + KR * i) * SB + 8 * (tid % CH)) = h[q];
+    }
+    if (do_cs && s * ROWS / 64 % p.sharers == at.tile_m) {
+#pragma unroll
+      for (int i = 0; i < DC; ++i) {
+        float v[8];
+        D::values(chunk(i), off + dvoff + i * dstep, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) cs[e] += v[e];
       }
-      u4 h[P];
-      split8<P>(v, h);
-#pragma unroll
-      for (int q = 0; q < P; ++q)
-        *reinterpret_cast<u4*>(b + q * ROWS * SB + ((tid + THREADS * i) / CH) * SB + 8 * (tid % CH)) = h[q];
     }
   };
 
@@ -321,30 +407,34 @@ __device__ __forceinline__ void planes_body(const Args& p, const Place& at, unsi
 #pragma unroll
         for (int t = 0; t < TM; ++t)
 #pragma unroll
-          for (int u = 0; u < TN; ++u)
-            acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fb[u]),
-                                                                __builtin_bit_cast(bf16x8, fa[t]), acc[t][u], 0, 0, 0);
+          for (int u = 0; u < TN; ++u) acc[t][u] = mfma<D::F16>(fa[t], fb[u], acc[t][u]);
       }
     }
   };
 
-  load(0);
-  store(0);
+  // Two stages a turn, without a branch between them: after one, the compiler
+  // would wait for all loads, not for those it needs.  Past the last stage rows
+  // are zeros (their loads have empty descriptors).
+  Raw r0, r1;
+  load(0, r0);
+  load(1, r1);
+  store(0, r0);
+  load(2, r0);
   __syncthreads();
-  for (int s = 0; s < stages; ++s) {
-    if (s + 1 < stages) load(s + 1);
+  auto stage = [&](int s, Raw& next) {
     compute(s);
-    if (s + 1 < stages) store(s + 1);
+    store(s + 1, next);
+    load(s + 3, next);
     __syncthreads();
+  };
+  for (int s = 0; s + 1 < stages; s += 2) {
+    stage(s, r1);
+    stage(s + 1, r0);
   }
+  if (stages & 1) compute(stages - 1);
+  __syncthreads();
   if (do_cs) store_shares<THREADS, CH>(p, cs, reinterpret_cast<float*>(smem), at, tid);
   store_c<TM, TN>(p, acc, at, wm, wn, g, r);
-}
-
-template <int DT, int BM, int BN, int WGM, int WGN>
-__global__ __launch_bounds__(64 * WGM * WGN) void mx_dw_planes_kernel(Args p) {
-  __shared__ __attribute__((aligned(16))) unsigned short smem[planes_lds<DT, BM, BN>()];
-  planes_body<DT, BM, BN, WGM, WGN>(p, place<BM, BN>(p), smem);
 }
 
 // ---------------------------------------------------------------- δ as it stands
@@ -363,11 +453,11 @@ __device__ __forceinline__ void direct_body(const Args& p, const Place& at, unsi
   constexpr int WAVES = WGM * WGN, THREADS = 64 * WAVES, ROWS = 64;
   constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   constexpr int STAGE = ROWS * (BM + BN);
-  constexpr int XC = ROWS * BM / 16 / THREADS;          // chunks of X a thread
   constexpr int LOADS = ROWS * BN * 2 / 1024 / WAVES;   // δ's loads a wave
   constexpr int RPL = 512 / BN;                         // rows a load
   constexpr int CH = BN / 8, KG = THREADS / CH;
-  static_assert(XC * THREADS * 16 == ROWS * BM && LOADS * WAVES * 1024 == ROWS * BN * 2, "loads split evenly");
+  static_assert(LOADS * WAVES * 1024 == ROWS * BN * 2 && THREADS % CH == 0 && KG * (ROWS / KG) == ROWS, "even split");
+  using X = XSide<ROWS, BM, THREADS>;
   static_assert(BM % 128 == 0 && BN % 128 == 0 && (RPL * WAVES) % 16 == 0, "swizzle period");
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -389,33 +479,16 @@ __device__ __forceinline__ void direct_body(const Args& p, const Place& at, unsi
     for (int i = 0; i < LOADS; ++i)
       rt_dev::dma16_at(rsrc, smem_at + 2 * ((s & 1) * STAGE + ROWS * BM) + 1024 * (i * WAVES + wave), voff + i * vstep);
   };
-  // X: a thread's chunks are 32 rows apart (of the 64 of a group), in the same
-  // columns, so one dword holds all their scales.  Rows past the slice's end are
-  // zeros; columns past X's last come from elsewhere, in rows of C that are not
-  // stored.
-  constexpr int XR = BM / 16;  // chunks a row
-  static_assert(THREADS / XR == 32 && XC == 2, "chunks of X");
-  const int xk = tid / XR, xvoff = xk * p.x_row + 16 * (tid % XR);
-  const int svoff = (tid % XR) / 8 * (p.x_groups * 256) + 4 * (16 * (tid % 8 / 2) + xk % 16);
-  u4 xw[XC];
-  unsigned xs;
-  auto load_x = [&](int s) {
-    const long long row = at.rb + (long long)s * ROWS, group = row / 64;
-    const long long first = (long long)(at.m0 / 128) * p.x_groups + group, all = (long long)(p.x_row / 128) * p.x_groups;
-    const __amdgpu_buffer_rsrc_t rsrc = bounded_rsrc(p.x + row * p.x_row + at.m0, (at.re - row) * p.x_row - at.m0);
-    const __amdgpu_buffer_rsrc_t srsrc = bounded_rsrc(p.x_scales + first * 256, (all - first) * 256);
-#pragma unroll
-    for (int i = 0; i < XC; ++i) xw[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, xvoff + i * 32 * p.x_row, 0, 0);
-    xs = __builtin_amdgcn_raw_buffer_load_b32(srsrc, svoff, 0, 0);
-  };
+  X xs;
+  xs.init(p, at, tid);
+  typename X::Raw xr;
+  auto load_x = [&](int s) { xs.load(p, at, s, xr); };
   auto store_x = [&](int s) {
-    unsigned short* a = smem + (s & 1) * STAGE + xk * BM + 16 * ((tid % XR) ^ hm(xk));
+    unsigned short* a = smem + (s & 1) * STAGE + xs.k * BM + 16 * ((tid % X::XR) ^ hm(xs.k));
 #pragma unroll
-    for (int i = 0; i < XC; ++i) {
+    for (int i = 0; i < X::CHUNKS; ++i) {
       u4 h[2];
-      // Absent rows have no scale either (their byte may be any).
-      const bool in = at.rb + (long long)s * ROWS + xk + 32 * i < at.re;
-      decode16<F16>(xw[i], in ? (xs >> (8 * (xk / 16 + 2 * i))) & 0xffu : 0u, h);
+      xs.template decode<F16>(at, s, xr, i, h);
       u4* to = reinterpret_cast<u4*>(a + 32 * i * BM);
       to[0] = h[0];
       to[1] = h[1];
@@ -451,14 +524,7 @@ __device__ __forceinline__ void direct_body(const Args& p, const Place& at, unsi
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
 #pragma unroll
-      for (int u = 0; u < TN; ++u) {
-        if constexpr (F16)
-          acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, cur[u]),
-                                                             __builtin_bit_cast(f16x8, fa[t]), acc[t][u], 0, 0, 0);
-        else
-          acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, cur[u]),
-                                                              __builtin_bit_cast(bf16x8, fa[t]), acc[t][u], 0, 0, 0);
-      }
+      for (int u = 0; u < TN; ++u) acc[t][u] = mfma<F16>(fa[t], cur[u], acc[t][u]);
       fa[t] = read_a(s, kk, t);
     }
     // Kept in this order: the scheduler would move the reads up, into new registers.
@@ -468,13 +534,14 @@ __device__ __forceinline__ void direct_body(const Args& p, const Place& at, unsi
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
     });
   };
-  const bool do_cs = p.shares != nullptr;
+  const bool do_cs = p.shares != nullptr && at.tile_m < p.sharers;
   float cs[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   auto colsum = [&](int s) {
     const unsigned short* b = smem + (s & 1) * STAGE + ROWS * BM;
     const int c = tid % CH;
 #pragma unroll
-    for (int k = tid / CH; k < ROWS; k += KG) {
+    for (int i = 0; i < ROWS / KG; ++i) {
+      const int k = tid / CH + KG * i;
       const u4 v = *reinterpret_cast<const u4*>(b + k * BN + 16 * ((c >> 1) ^ hm(k)) + 8 * (c & 1));
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -485,28 +552,32 @@ __device__ __forceinline__ void direct_body(const Args& p, const Place& at, unsi
     }
   };
 
-  // Past the last stage rows are zeros: loaded, decoded, never multiplied.
+  // Past the last stage rows are zeros: decoded, never multiplied.
   issue(0);
   load_x(0);
   wait_vm<0>();
   store_x(0);
-  issue(1);
-  load_x(1);
-  wait_vm<0>();
-  store_x(1);
-  load_x(2);
+  if (stages > 1) {
+    issue(1);
+    load_x(1);
+    wait_vm<0>();
+    store_x(1);
+    load_x(2);
+  }
   barrier_lds();
   read_b(0, 0, fb0);
 #pragma unroll
   for (int t = 0; t < TM; ++t) fa[t] = read_a(0, 0, t);
   for (int s = 0; s < stages; ++s) {
     k_step(fb0, fb1, s, 1);
-    if (do_cs && s % p.tiles_m == at.tile_m) colsum(s);
+    if (do_cs && s % p.sharers == at.tile_m) colsum(s);
     wait_vm<0>();
     barrier_lds();
-    if (s + 2 < stages) issue(s + 2);
-    store_x(s + 2);
-    load_x(s + 3);
+    if (s + 2 < stages) {
+      issue(s + 2);
+      store_x(s + 2);
+      load_x(s + 3);
+    }
     k_step(fb1, fb0, s + 1, 0);
   }
   __syncthreads();
@@ -514,61 +585,111 @@ __device__ __forceinline__ void direct_body(const Args& p, const Place& at, unsi
   store_c<TM, TN>(p, acc, at, wm, wn, g, r);
 }
 
-template <bool F16, int BM, int BN, int WGM, int WGN>
-__global__ __launch_bounds__(64 * WGM * WGN) void mx_dw_kernel(Args p) {
-  constexpr int LDS = 2 * 64 * (BM + BN), OTHER = F16 ? planes_lds<RT_F16, BM, BN>() : 0;
-  __shared__ __attribute__((aligned(16))) unsigned short smem[LDS > OTHER ? LDS : OTHER];
-  const Place at = place<BM, BN>(p);
-  if constexpr (F16) {
-    // Scales that f16 holds: 448·2^7 and 2^-9·2^-15 are f16 values.  A byte of 0
-    // is a block of zeros (or of values below 2^-118, which count as zeros).
-    int bad = 0;
-    const long long g0 = at.rb / 64, n = (at.re + 63) / 64 - g0;
-    for (int step = at.m0 / 128; step < min(at.m0 + BM, p.x_row) / 128; ++step) {
-      const unsigned* sc = reinterpret_cast<const unsigned*>(p.x_scales) + ((long long)step * p.x_groups + g0) * 64;
-      for (long long i = threadIdx.x; i < n * 64; i += 64 * WGM * WGN) {
-        const unsigned w = sc[i];
+// Whether f16 holds the values of the block's part of X: scales from 2^-15 to
+// 2^7 (448·2^7 and 2^-9·2^-15 are f16 values).  A byte of 0 is a block of zeros
+// (or of values below 2^-118, which count as zeros).
+template <int BM, int THREADS>
+__device__ inline bool f16_holds(const Args& p, const Place& at) {
+  int bad = 0;
+  const long long g0 = at.rb / 64, n = (at.re + 63) / 64 - g0;
+  for (int step = at.m0 / 128; 128 * step < min(at.m0 + BM, p.x_row); ++step) {
+    const unsigned* sc = reinterpret_cast<const unsigned*>(p.x_scales) + ((long long)step * p.x_groups + g0) * 64;
+    for (long long i = threadIdx.x; i < n * 64; i += THREADS) {
+      const unsigned w = sc[i];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned b = (w >> (8 * e)) & 0xffu;
-          bad |= b != 0 && (b < 112 || b > 134);
-        }
+      for (int e = 0; e < 4; ++e) {
+        const unsigned b = (w >> (8 * e)) & 0xffu;
+        bad |= b != 0 && (b < 112 || b > 134);
       }
     }
-    if (__syncthreads_or(bad)) return planes_body<RT_F16, BM, BN, WGM, WGN>(p, at, smem);
   }
-  direct_body<F16, BM, BN, WGM, WGN>(p, at, smem);
+  return !__syncthreads_or(bad);
+}
+
+constexpr int larger(int a, int b) { return a > b ? a : b; }
+
+// 128 x 128 with four waves, 64 x 64 with two.
+template <int KIND, int TILE>
+__global__ __launch_bounds__(2 * TILE, 2) void mx_dw_staged_kernel(Args p) {
+  constexpr int OTHER = KIND == kF16 ? kF16Planes : KIND, WGN = TILE / 64;
+  __shared__ __attribute__((aligned(16))) unsigned short smem[larger(staged_lds<KIND, TILE, TILE>(), staged_lds<OTHER, TILE, TILE>())];
+  const Place at = place<TILE, TILE>(p);
+  if constexpr (KIND == kF16) {
+    if (!f16_holds<TILE, 2 * TILE>(p, at)) return staged_body<kF16Planes, TILE, TILE, 2, WGN>(p, at, smem);
+  }
+  staged_body<KIND, TILE, TILE, 2, WGN>(p, at, smem);
+}
+
+template <bool F16>
+__global__ __launch_bounds__(512) void mx_dw_direct_kernel(Args p) {
+  __shared__ __attribute__((aligned(16))) unsigned short smem[larger(2 * 64 * 512, staged_lds<kF16Planes, 256, 256>())];
+  const Place at = place<256, 256>(p);
+  if constexpr (F16) {
+    if (!f16_holds<256, 512>(p, at)) return staged_body<kF16Planes, 256, 256, 2, 4>(p, at, smem);
+  }
+  direct_body<F16, 256, 256, 2, 4>(p, at, smem);
 }
 
 struct Plan {
-  bool direct;  // δ straight into LDS
-  int tile;     // 256 or 128, square
+  int tile;  // 256 (δ straight into LDS), 128 or 64 (through registers), square
   long long tiles_m, tiles_n, rows_per_split;
-  int splits;
+  int splits, sharers;
 };
 
-// Slices of rows where the tiles of C alone do not fill the chip: up to 256
-// blocks of 256 x 256 (one a CU), 512 of 128 x 128 (two).
+// The tile and the slices of rows, by what they are expected to take.  A block
+// alone on its CU takes `alone` a stage (latencies), several share the CU's
+// throughput (`each`); slices write and read a plane of C each (4 TB/s, counted
+// once each way, and a launch).  Measured, us: 2048 rows, 1024 x 1024, bf16: 64
+// tiles unsplit 32.6, 3 slices 23.9, 8 30; 128 tiles 4 slices 25.8, unsplit 41.8;
+// f32: 64 tiles 4 slices 33.2, unsplit 62.3.  600 rows, 2000 x 1500, bf16: 64
+// tiles 17.9 unsplit, 29 in 2 slices.  5000 rows, 200 x 64, bf16: 64 tiles 69
+// unsplit, 9.9 in 32 slices.  8192 rows, 4096 x 4096, bf16: 239 with 256 tiles,
+// 355 with 128.
 Plan plan(const rt::MxTensor& x, const void* delta, int dtype, long long N) {
-  Plan q;
-  q.direct = dtype != RT_F32 && N % 8 == 0 && (reinterpret_cast<uintptr_t>(delta) & 15) == 0 && N <= (1LL << 23) &&
-             x.cols <= (1LL << 23) && x.rows <= (1LL << 28);  // offsets of a stage below 2^31 bytes
-  auto tiles = [&](int t) { return ((x.cols + t - 1) / t) * ((N + t - 1) / t); };
-  auto splits = [&](int t, long long blocks, long long rows) {
-    return std::max<long long>(1, std::min(blocks / std::max<long long>(tiles(t), 1), x.rows / rows));
+  struct Tile {
+    int size;
+    float alone, each;  // us a stage of a block
   };
-  q.tile = q.direct && tiles(256) * splits(256, 256, 1024) >= 192 ? 256 : 128;
-  const long long want = q.tile == 256 ? splits(256, 256, 1024) : splits(128, 512, 256);
-  q.tiles_m = (x.cols + q.tile - 1) / q.tile;
-  q.tiles_n = (N + q.tile - 1) / q.tile;
-  q.rows_per_split = ((x.rows + want - 1) / want + 63) / 64 * 64;
-  q.splits = (int)((x.rows + q.rows_per_split - 1) / q.rows_per_split);
-  return q;
+  static constexpr Tile kTiles[3] = {{64, 0.9f, 0.35f}, {128, 1.2f, 0.85f}, {256, 1.8f, 1.8f}};
+  // 256 tiles take rows of δ by whole 16-byte chunks (and a step's scales below
+  // 2^31 bytes).
+  const bool direct = dtype != RT_F32 && N % 8 == 0 && (reinterpret_cast<uintptr_t>(delta) & 15) == 0 &&
+                      x.rows <= (1LL << 28);
+  const int stage_rows = dtype == RT_F32 ? 32 : 64;
+  const float plane_us = 4.0f * (float)x.cols * (float)N / 4e6f;
+  Plan best{};
+  float best_us = 0;
+  for (int t = 0; t < (direct ? 3 : 2); ++t) {
+    const Tile& tile = kTiles[t];
+    const long long tm = (x.cols + tile.size - 1) / tile.size, tn = (N + tile.size - 1) / tile.size;
+    for (long long want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128}) {
+      if (want > 1 && want * 64 > x.rows) break;
+      const long long per = ((x.rows + want - 1) / want + 63) / 64 * 64, splits = (x.rows + per - 1) / per;
+      const long long on_cu = (tm * tn * splits + 255) / 256;
+      const float us = (float)((per + stage_rows - 1) / stage_rows) * std::max(tile.alone, (float)on_cu * tile.each) +
+                       (splits > 1 ? 2.0f + 2.0f * (float)splits * plane_us : plane_us);
+      if (best_us == 0 || us < best_us) {
+        best_us = us;
+        best = Plan{tile.size, tm, tn, per, (int)splits, 0};
+      }
+    }
+  }
+  // The bias gradient: over a long slice the tile rows share its pieces, over a
+  // short one the first adds them all, which saves the launch that adds shares
+  // (37 rows, 1024 x 1000, bf16: 7.2 us and 2.2 for that launch; 4.4 without).
+  best.sharers = best.rows_per_split > 1024 ? (int)best.tiles_m : 1;
+  return best;
+}
+
+template <int KIND>
+void launch_staged(hipStream_t s, const Args& p, const Plan& q, dim3 grid) {
+  if (q.tile == 128) rt::launch(mx_dw_staged_kernel<KIND, 128>, grid, dim3(256), 0, s, p);
+  else rt::launch(mx_dw_staged_kernel<KIND, 64>, grid, dim3(128), 0, s, p);
 }
 
 size_t plane_elems(const Plan& q, long long K, long long N) { return q.splits > 1 ? (size_t)q.splits * K * N : 0; }
 size_t share_elems(const Plan& q, long long N) {
-  return q.splits * q.tiles_m > 1 ? (size_t)q.splits * q.tiles_m * N : 0;
+  return q.splits * q.sharers > 1 ? (size_t)q.splits * q.sharers * N : 0;
 }
 
 }  // namespace
@@ -579,7 +700,7 @@ size_t mx_dw_scratch_elems(const MxTensor& x, const void* delta, int delta_dtype
   if (x.rows == 0 || x.cols == 0) return 0;
   const Plan q = plan(x, delta, delta_dtype, N);
   size_t n = plane_elems(q, x.cols, N);
-  if (colsum) n += share_elems(q, N) + (q.splits == 1 ? colsum_scratch_elems((int)q.tiles_m, (int)N, RT_F32) : 0);
+  if (colsum) n += share_elems(q, N) + (q.splits == 1 ? colsum_scratch_elems(q.sharers, (int)N, RT_F32) : 0);
   return n;
 }
 
@@ -593,6 +714,7 @@ hipError_t mx_dw_launch(hipStream_t s, const MxTensor& x, const void* delta, int
   p.x_scales = x.scales;
   p.delta = delta;
   p.c = q.splits > 1 ? scratch : C;
+  p.sharers = q.sharers;
   p.shares = !colsum ? nullptr : shares ? scratch + planes : colsum;
   p.rows = x.rows;
   p.K = (int)x.cols;
@@ -604,26 +726,19 @@ hipError_t mx_dw_launch(hipStream_t s, const MxTensor& x, const void* delta, int
   p.tiles_m = (int)q.tiles_m;
   p.tiles_n = (int)q.tiles_n;
   const dim3 grid((unsigned)(q.tiles_m * q.tiles_n * q.splits));
-  if (q.direct && q.tile == 256) {
-    if (delta_dtype == RT_F16) rt::launch(mx_dw_kernel<true, 256, 256, 2, 4>, grid, dim3(512), 0, s, p);
-    else rt::launch(mx_dw_kernel<false, 256, 256, 2, 4>, grid, dim3(512), 0, s, p);
-  } else if (q.direct) {
-    if (delta_dtype == RT_F16) rt::launch(mx_dw_kernel<true, 128, 128, 2, 2>, grid, dim3(256), 0, s, p);
-    else rt::launch(mx_dw_kernel<false, 128, 128, 2, 2>, grid, dim3(256), 0, s, p);
-  } else if (delta_dtype == RT_F32) {
-    rt::launch(mx_dw_planes_kernel<RT_F32, 128, 128, 2, 2>, grid, dim3(256), 0, s, p);
-  } else if (delta_dtype == RT_F16) {
-    rt::launch(mx_dw_planes_kernel<RT_F16, 128, 128, 2, 2>, grid, dim3(256), 0, s, p);
-  } else {
-    rt::launch(mx_dw_planes_kernel<RT_BF16, 128, 128, 2, 2>, grid, dim3(256), 0, s, p);
-  }
+  if (q.tile == 256)
+    delta_dtype == RT_F16 ? rt::launch(mx_dw_direct_kernel<true>, grid, dim3(512), 0, s, p)
+                          : rt::launch(mx_dw_direct_kernel<false>, grid, dim3(512), 0, s, p);
+  else if (delta_dtype == RT_F32) launch_staged<kF32>(s, p, q, grid);
+  else if (delta_dtype == RT_F16) launch_staged<kF16>(s, p, q, grid);
+  else launch_staged<kBf16>(s, p, q, grid);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (q.splits > 1)
     return splitk_reduce_launch(s, scratch, q.splits, p.split_stride, p.K, p.N, C, RT_F32, p.N, RT_EPI_NONE, nullptr,
-                                nullptr, RT_F32, p.shares, colsum, colsum ? p.tiles_m : 0);
+                                nullptr, RT_F32, p.shares, colsum, colsum ? p.sharers : 0);
   if (colsum && shares)
-    return colsum_launch(s, p.shares, RT_F32, p.tiles_m, p.N, colsum, scratch + planes + shares,
+    return colsum_launch(s, p.shares, RT_F32, p.sharers, p.N, colsum, scratch + planes + shares,
                          scratch_elems - planes - shares);
   return hipSuccess;
 }

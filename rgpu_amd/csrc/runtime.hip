@@ -554,6 +554,8 @@ static int mx_gemm(rt_ctx* c, rt_layout layout, const rt_buf* a, const rt_buf* b
   if (out->dtype != RT_F32) return fail(c, RT_ERR_DTYPE, "the gradient from an 8-bit input is f32");
   if (epi != RT_EPI_NONE) return fail(c, RT_ERR_INVALID, "the TN product of an 8-bit A has no epilogue");
   if (colsum && (colsum->dtype != RT_F32 || colsum->n != N)) return fail(c, RT_ERR_SHAPE, "colsum must be f32 [%zu]", N);
+  // A stage of 64 rows stays below 2^31 bytes.
+  if (M > kMxMaxCols || N > kMxMaxCols) return fail(c, RT_ERR_SHAPE, "the gradient from an 8-bit input is at most 2^22 wide");
   if (N == 0) return RT_OK;
   if (M == 0 || K == 0) {  // no input column: the bias gradient alone; no row: zeros
     if (M > 0)

@@ -82,6 +82,10 @@ def test_refusals(gpu):
     assert status(gpu.matmul_at_b, m8, f(9, 8), dw) == "RT_ERR_SHAPE"
     assert status(gpu.matmul_at_b, m8, f(8, 8), dw, f(9)) == "RT_ERR_SHAPE"
     assert status(gpu.gemm, G.TN, m8, f(8, 8), dw, G.EPI_BIAS, f(8)) == "RT_ERR_INVALID"
+    wide = gpu.zeros((1, 2 ** 22 + 1), G.MXFP8)
+    assert status(gpu.matmul_at_b, wide, f(1, 1), f(2 ** 22 + 1, 1)) == "RT_ERR_SHAPE"
+    assert status(gpu.matmul_at_b, gpu.zeros((1, 1), G.MXFP8), f(1, 2 ** 22 + 1), f(1, 2 ** 22 + 1)) == "RT_ERR_SHAPE"
+    assert status(gpu.gemm, G.NT, wide, gpu.zeros((1, 2 ** 22 + 1), G.MXFP4), f(1, 1)) == "RT_ERR_SHAPE"
     assert status(gpu.linear_backward, m4, f(8, 8), f(40, 8), f(8, 40), dw) == "RT_ERR_DTYPE"
     # masks
     assert status(gpu.matmul_a_bt, f(8, 5), f(40, 5), f(8, 40), m4) == "RT_ERR_DTYPE"
@@ -373,6 +377,28 @@ def test_dw_f16_scales_beyond_f16(gpu, rows, N):
     check_dw(gpu, rows, 300, N, "f16", x=x)
     x[:, 64:96], x[:, 128:160] = 65504.0, 2.0 ** -24  # the largest and the smallest of f16
     check_dw(gpu, rows, 300, N, "f16", x=x)
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPE))
+@pytest.mark.parametrize("N", [1, 7, 63, 129])
+def test_dw_from_any_place_in_memory(gpu, dtype, N):
+    """A gradient that starts on any element of its allocation, with values before and behind it that are not its own."""
+    rng = np.random.default_rng(N)
+    rows, K = 131, 40
+    x = np.maximum(X.values(rng, rows, K), 0)
+    q, xv = mx_upload(gpu, x, G.MXFP8)
+    t = torch.full((rows * N + 16,), float("nan"), device="cuda",
+                   dtype={"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype])
+    for start in (0, 1, 2, 3, 5, 8):
+        d64 = rounded(rng.normal(size=(rows, N)), DTYPE[dtype])
+        t.fill_(float("nan"))
+        t[start:start + rows * N] = torch.from_numpy(d64.reshape(-1)).to(t)
+        torch.cuda.synchronize()
+        d = gpu.wrap(t.data_ptr() + start * t.element_size(), (rows, N), DTYPE[dtype], owner=t)
+        dw, db = gpu.empty((K, N)), gpu.empty((1, N))
+        gpu.matmul_at_b(q, d, dw, colsum=db)
+        assert np.all(np.abs(gpu.download(dw) - xv.T @ d64) <= (3 * rows + 40) * 2.0 ** -23 * (np.abs(xv).T @ np.abs(d64)))
+        assert np.all(np.abs(gpu.download(db)[0] - d64.sum(0)) <= (rows + 8) * 2.0 ** -24 * np.abs(d64).sum(0))
 
 
 def test_dw_absent_rows_have_no_scale(gpu):
