@@ -111,7 +111,19 @@ __device__ inline __amdgpu_buffer_rsrc_t bounded_rsrc(const void* base, long lon
                                            (int)max(0LL, min(bytes, 0x7ffffff0LL)), 0x00020000);
 }
 
-// X of a stage: a thread's chunks of 16 codes are 32 rows apart, in the same
+// What is left of an operand from the next stage on.
+struct Cursor {
+  const char* base;
+  long long left, step;  // bytes to the slice's end, bytes a stage
+  __device__ inline __amdgpu_buffer_rsrc_t next() {
+    const __amdgpu_buffer_rsrc_t r = bounded_rsrc(base, left);
+    base += step;
+    left -= step;
+    return r;
+  }
+};
+
+// X by stages: a thread's chunks of 16 codes are 32 rows apart, in the same
 // columns; the dword that holds the scale of one holds those of all (of the
 // 64-row group).  Rows past the slice's end are zeros; columns past X's last come
 // from elsewhere, in rows of C that are not stored.
@@ -123,28 +135,36 @@ struct XSide {
     u4 w[CHUNKS];
     unsigned scales;
   };
-  int k, voff, svoff;  // row and column of the first chunk
+  Cursor codes, scales;
+  int k, voff, svoff, vstep, rows;  // row and place of the first chunk; rows of the slice
   __device__ inline void init(const Args& p, const Place& at, int tid) {
     const int c = at.m0 % 128 / 16 + tid % XR;  // chunk of its 128 columns, and beyond
     k = tid / XR;
     voff = k * p.x_row + 16 * (tid % XR);
+    vstep = 32 * p.x_row;
     svoff = c / 8 * (p.x_groups * 256) + 4 * (16 * (c % 8 / 2) + k % 16);
+    rows = (int)(at.re - at.rb);
+    codes = Cursor{reinterpret_cast<const char*>(p.x + at.rb * p.x_row + at.m0), (long long)rows * p.x_row - at.m0,
+                   (long long)ROWS * p.x_row};
+    const long long first = (long long)(at.m0 / 128) * p.x_groups + at.rb / 64;
+    scales = Cursor{reinterpret_cast<const char*>(p.x_scales + first * 256),
+                    ((long long)(p.x_row / 128) * p.x_groups - first) * 256, 256};
   }
-  __device__ inline void load(const Args& p, const Place& at, int s, Raw& x) const {
-    const long long row = at.rb + (long long)s * ROWS, group = row / 64;
-    const long long first = (long long)(at.m0 / 128) * p.x_groups + group, all = (long long)(p.x_row / 128) * p.x_groups;
-    const __amdgpu_buffer_rsrc_t rsrc = bounded_rsrc(p.x + row * p.x_row + at.m0, (at.re - row) * p.x_row - at.m0);
-    const __amdgpu_buffer_rsrc_t srsrc = bounded_rsrc(p.x_scales + first * 256, (all - first) * 256);
+  // The next stage; s: its number.
+  __device__ inline void load(int s, Raw& x) {
+    const __amdgpu_buffer_rsrc_t rsrc = codes.next();
 #pragma unroll
-    for (int i = 0; i < CHUNKS; ++i) x.w[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, voff + i * 32 * p.x_row, 0, 0);
+    for (int i = 0; i < CHUNKS; ++i) x.w[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, voff + i * vstep, 0, 0);
+    const __amdgpu_buffer_rsrc_t srsrc = bounded_rsrc(scales.base, scales.left);
     x.scales = __builtin_amdgcn_raw_buffer_load_b32(srsrc, svoff, 0, 0);
+    if (ROWS == 64 || (s & 1)) scales.next();  // a group is 64 rows
   }
   // Chunk i as 16 halves.  Absent rows have no scale either (their byte may be any).
   template <bool F16>
-  __device__ inline void decode(const Place& at, int s, const Raw& x, int i, u4 (&h)[2]) const {
-    const long long row = at.rb + (long long)s * ROWS + k + 32 * i;
-    const unsigned byte = (x.scales >> (8 * ((int)row % 64 / 16))) & 0xffu;
-    decode16<F16>(x.w[i], row < at.re ? byte : 0u, h);
+  __device__ inline void decode(int s, const Raw& x, int i, u4 (&h)[2]) const {
+    const int row = s * ROWS + k + 32 * i;
+    const unsigned byte = (x.scales >> (8 * (row % 64 / 16))) & 0xffu;
+    decode16<F16>(x.w[i], row < rows ? byte : 0u, h);
   }
 };
 
@@ -185,6 +205,17 @@ __device__ __forceinline__ void store_c(const Args& p, const f4 (&acc)[TM][TN], 
     }
   });
 }
+
+// Whose turn a 64-row piece's column sums are: tile row t's, pieces t, t +
+// sharers, ...
+struct Turn {
+  int left, sharers;  // pieces until the next one of this tile row
+  __device__ inline bool take(bool done) {  // done: the piece ends here
+    const bool mine = left == 0;
+    if (done) left = mine ? sharers - 1 : left - 1;
+    return mine;
+  }
+};
 
 // Each thread's sums of 8 columns (chunk tid % CH), over the threads that share
 // them, in a fixed order.  smem: THREADS * 8 floats that nothing else uses.
@@ -316,63 +347,57 @@ __device__ __forceinline__ void staged_body(const Args& p, const Place& at, unsi
 
   X xs;
   xs.init(p, at, tid);
-  // δ is addressed from the dword that holds its slice's first value of the
-  // stage, to the one that holds its last; columns past N are the next row's.
-  const unsigned dvoff = (unsigned)D::SIZE * ((unsigned)(tid / CH) * p.N + 8 * (tid % CH)), dstep = D::SIZE * KR * p.N;
-  auto delta_at = [&](int s) {  // address of the stage's first value
-    return reinterpret_cast<uintptr_t>(p.delta) +
-           (unsigned long long)D::SIZE * ((at.rb + (long long)s * ROWS) * p.N + at.n0);
-  };
+  // δ is addressed from the dword that holds the slice's first value (every
+  // stage's then starts at the same place of its dword) to the one that holds its
+  // last; columns past N are the next row's.  Half of the last dword may be a
+  // value of an absent row, whose chunks are therefore sent past the end.
+  const uintptr_t from = reinterpret_cast<uintptr_t>(p.delta) + (unsigned long long)D::SIZE * (at.rb * p.N + at.n0);
+  const unsigned odd = (unsigned)(from & 3);
+  const unsigned dvoff = odd + (unsigned)D::SIZE * ((unsigned)(tid / CH) * p.N + 8 * (tid % CH));
+  const unsigned dstep = D::SIZE * KR * p.N;
+  Cursor dc{reinterpret_cast<const char*>(from - odd),
+            (D::SIZE * ((at.re - at.rb) * p.N - at.n0) + (long long)odd + 3) & ~3LL, (long long)D::SIZE * ROWS * p.N};
   struct Raw {
     typename X::Raw x;
     typename D::Raw d[DC];
   };
   auto load = [&](int s, Raw& raw) {
-    xs.load(p, at, s, raw.x);
-    const uintptr_t from = delta_at(s), base = from & ~(uintptr_t)3;
-    const long long rows = at.re - at.rb - (long long)s * ROWS;
-    const long long bytes = rows > 0 ? (D::SIZE * (rows * p.N - at.n0) + (long long)(from - base) + 3) & ~3LL : 0;
-    const __amdgpu_buffer_rsrc_t rsrc = bounded_rsrc(reinterpret_cast<const void*>(base), bytes);
+    xs.load(s, raw.x);
+    const __amdgpu_buffer_rsrc_t rsrc = dc.next();
 #pragma unroll
-    for (int i = 0; i < DC; ++i) raw.d[i] = D::load(rsrc, (unsigned)(from - base) + dvoff + i * dstep);
+    for (int i = 0; i < DC; ++i) {
+      const bool in = D::SIZE == 4 || s * ROWS + tid / CH + KR * i < xs.rows;
+      raw.d[i] = D::load(rsrc, in ? dvoff + i * dstep : 0x7fffff00u);
+    }
   };
   const bool do_cs = p.shares != nullptr && at.tile_m < p.sharers;
   float cs[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  Turn turn{at.tile_m, p.sharers};
   auto store = [&](int s, const Raw& raw) {
     unsigned short* a = smem + (s & 1) * STAGE;
     unsigned short* b = a + ROWS * SA;
 #pragma unroll
     for (int i = 0; i < X::CHUNKS; ++i) {
       u4 h[2];
-      xs.template decode<D::F16>(at, s, raw.x, i, h);
+      xs.template decode<D::F16>(s, raw.x, i, h);
       u4* to = reinterpret_cast<u4*>(a + (xs.k + 32 * i) * SA + 16 * (tid % X::XR));
       to[0] = h[0];
       to[1] = h[1];
     }
-    const unsigned off = (unsigned)(delta_at(s) & 3);
-    // Half of the last dword may be a value of an absent row.
-    auto chunk = [&](int i) {
-      typename D::Raw d = raw.d[i];
-      if constexpr (D::SIZE == 2) {
-        const bool in = at.rb + (long long)s * ROWS + tid / CH + KR * i < at.re;
-        d.w = in ? d.w : u4{0u, 0u, 0u, 0u};
-        d.last = in ? d.last : 0u;
-      }
-      return d;
-    };
 #pragma unroll
     for (int i = 0; i < DC; ++i) {
       u4 h[P];
-      D::planes(chunk(i), off + dvoff + i * dstep, h);
+      D::planes(raw.d[i], dvoff + i * dstep, h);
 #pragma unroll
       for (int q = 0; q < P; ++q)
         *reinterpret_cast<u4*>(b + q * ROWS * SB + (tid / CH + KR * i) * SB + 8 * (tid % CH)) = h[q];
     }
-    if (do_cs && s * ROWS / 64 % p.sharers == at.tile_m) {
+    const bool mine = turn.take(ROWS == 64 || (s & 1));
+    if (do_cs && mine) {
 #pragma unroll
       for (int i = 0; i < DC; ++i) {
         float v[8];
-        D::values(chunk(i), off + dvoff + i * dstep, v);
+        D::values(raw.d[i], dvoff + i * dstep, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) cs[e] += v[e];
       }
@@ -470,11 +495,11 @@ __device__ __forceinline__ void direct_body(const Args& p, const Place& at, unsi
   const int k0 = RPL * wave + lane / CH, slot = lane % CH;
   const int voff = 2 * (k0 * p.N + 16 * ((slot >> 1) ^ hm(k0)) + 8 * (slot & 1)), vstep = 2 * RPL * WAVES * p.N;
   const unsigned smem_at = rt_dev::lds_offset(smem);
+  // The slice's rows end where its bytes do: what follows arrives as zeros.
+  Cursor dc{reinterpret_cast<const char*>(static_cast<const unsigned short*>(p.delta) + at.rb * p.N + at.n0),
+            2 * ((at.re - at.rb) * p.N - at.n0), 2LL * ROWS * p.N};
   auto issue = [&](int s) {
-    const long long row = at.rb + (long long)s * ROWS;
-    const unsigned short* src = static_cast<const unsigned short*>(p.delta) + row * p.N + at.n0;
-    // The slice's rows end here: what follows arrives as zeros.
-    const __amdgpu_buffer_rsrc_t rsrc = bounded_rsrc(src, 2 * ((at.re - row) * p.N - at.n0));
+    const __amdgpu_buffer_rsrc_t rsrc = dc.next();
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
       rt_dev::dma16_at(rsrc, smem_at + 2 * ((s & 1) * STAGE + ROWS * BM) + 1024 * (i * WAVES + wave), voff + i * vstep);
@@ -482,13 +507,13 @@ __device__ __forceinline__ void direct_body(const Args& p, const Place& at, unsi
   X xs;
   xs.init(p, at, tid);
   typename X::Raw xr;
-  auto load_x = [&](int s) { xs.load(p, at, s, xr); };
+  auto load_x = [&](int s) { xs.load(s, xr); };
   auto store_x = [&](int s) {
     unsigned short* a = smem + (s & 1) * STAGE + xs.k * BM + 16 * ((tid % X::XR) ^ hm(xs.k));
 #pragma unroll
     for (int i = 0; i < X::CHUNKS; ++i) {
       u4 h[2];
-      xs.template decode<F16>(at, s, xr, i, h);
+      xs.template decode<F16>(s, xr, i, h);
       u4* to = reinterpret_cast<u4*>(a + 32 * i * BM);
       to[0] = h[0];
       to[1] = h[1];
@@ -536,6 +561,7 @@ __device__ __forceinline__ void direct_body(const Args& p, const Place& at, unsi
   };
   const bool do_cs = p.shares != nullptr && at.tile_m < p.sharers;
   float cs[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  Turn turn{at.tile_m, p.sharers};
   auto colsum = [&](int s) {
     const unsigned short* b = smem + (s & 1) * STAGE + ROWS * BM;
     const int c = tid % CH;
@@ -570,7 +596,8 @@ __device__ __forceinline__ void direct_body(const Args& p, const Place& at, unsi
   for (int t = 0; t < TM; ++t) fa[t] = read_a(0, 0, t);
   for (int s = 0; s < stages; ++s) {
     k_step(fb0, fb1, s, 1);
-    if (do_cs && s % p.sharers == at.tile_m) colsum(s);
+    const bool mine = turn.take(true);
+    if (do_cs && mine) colsum(s);
     wait_vm<0>();
     barrier_lds();
     if (s + 2 < stages) {
