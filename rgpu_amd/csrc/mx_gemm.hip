@@ -14,7 +14,7 @@
 // f32 additions.  For a bf16 C it goes in whole (SPLIT false): what is dropped
 // is at most 2^-13 of a neighbouring product, whose 8-bit factor was itself
 // rounded by up to 2^-5 of it, and half the work is saved (8192 x 4096, K 4096:
-// 208 us split, 121 whole).
+// 193 us split, 116 whole).
 //
 // What a lane holds.  Lane (g, r), g = lane / 16, r = lane % 16, of an operand
 // of 16 rows takes row r: the 4-bit codes of columns 32 g .. 32 g + 31 (16
@@ -456,22 +456,32 @@ hipError_t launch_tiles(hipStream_t s, Args p) {
   return hipGetLastError();
 }
 
-// A product of more rows.
+// Tiles by what fills the chip.  256 x 256 (4 bits) has a CU to itself, so it
+// takes whole rounds of 256, or a last one that leaves no more than a third of
+// all places idle (K 4096, us with 256 and 128 tiles: 8192 x 4096, 512 blocks, 80
+// and 93; 6912 x 4864, 513 blocks, 104 and 110; 4608 x 4096, 288 blocks, 66 and
+// 56).  128 x 128, two a CU, from 208 blocks on (1800 x 1800, K 2000, 225 blocks,
+// 8 bits: 13.2 and 13.9 with 64 tiles; 700 x 4096, K 1000, 192 blocks: 12.0 and
+// 10.6).  For 8 bits larger tiles were no faster (256 x 128, 8192 x 4096, K 4096:
+// 119.7 and 115.9 with 128).
 template <int ABITS, bool SPLIT>
 hipError_t launch_many(hipStream_t s, const Args& p) {
-  auto tiles = [&](int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+  auto tiles = [&](int t) { return (long long)((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
   if constexpr (ABITS == 4) {
-    if (tiles(256, 256) >= 256) return launch_tiles<4, false, 256, 256, 2, 4, 4>(s, p);
-  } else {
-    if (tiles(256, 128) >= 256) return launch_tiles<8, SPLIT, 256, 128, 4, 2, 3>(s, p);
+    const long long t = tiles(256), places = (t + 255) / 256 * 256;
+    if (t >= 256 && 2 * places <= 3 * t) return launch_tiles<4, false, 256, 256, 2, 4, 4>(s, p);
   }
-  if (tiles(128, 128) >= 128) return launch_tiles<ABITS, SPLIT, 128, 128, 2, 2, 3>(s, p);
+  if (tiles(128) >= 208) return launch_tiles<ABITS, SPLIT, 128, 128, 2, 2, 3>(s, p);
   return launch_tiles<ABITS, SPLIT, 64, 64, 2, 2, 4>(s, p);
 }
 
+// Few rows stay with the kernel that reads B once and A again for every 16
+// columns, up to 48, or 64 over a short K (N 4096, 8 bits, us there and with 64
+// tiles: 16 rows, K 4096, 5.0 and 8.0; 33 rows 7.7 and 8.1; 64 rows 11.2 and 8.1,
+// K 1024 5.4 and 5.7).
 template <int ABITS>
 hipError_t launch(hipStream_t s, const Args& p) {
-  if (p.M <= 64) {
+  if (p.M <= 48 || (p.M <= 64 && p.steps <= 8)) {
     const dim3 grid((unsigned)((p.N + 15) / 16)), block(64 * kRowWaves);
     const int tm = (p.M + 15) / 16;
     if (tm == 1) rt::launch(mx_rows_kernel<ABITS, 1>, grid, block, 0, s, p);

@@ -251,10 +251,10 @@ def check_product(gpu, M, N, K, fa, out, epi, seed=0):
     # K + 1 additions in f32, each off by at most one unit in the last place (2^-23) of what is summed so far, and
     # for bf16 one rounding of the result
     tol = (K + 8) * 2.0 ** -23 * size + (2.0 ** -8 * np.abs(want) if out == "bf16" else 0)
-    # An 8-bit A for a bf16 C of more than 64 rows: the matrix unit adds eight products in a window down to 2^-13 of the
+    # An 8-bit A for a bf16 C of more than 48 rows: the matrix unit adds eight products in a window down to 2^-13 of the
     # power of two of the largest, so each of the seven others loses less than 2^-13 of the largest, and an eight less
     # than 7 · 2^-13 of the sum of its sizes.
-    if fa == "fp8" and out == "bf16" and M > 64:
+    if fa == "fp8" and out == "bf16" and M > 48:
         tol = tol + 7 * 2.0 ** -13 * size
     err = np.abs(gpu.download_f32(c).astype(np.float64) - want)
     assert np.all(err <= tol), (err.max(), np.argwhere(err > tol)[:4])
