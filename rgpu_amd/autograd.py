@@ -42,7 +42,8 @@ from typing import Callable, Dict, List, Optional, Sequence, Tuple, Union
 import numpy as np
 
 from .gpu import (EPI_BIAS, EPI_BIAS_RELU, LOSS_BCE, LOSS_MAE, LOSS_SOFTMAX_XENT_LOGITS,
-                  LOSS_SOFTMAX_XENT_LOGITS_MEAN, NN, NT, TN, Gpu, GpuTensor, RtError, upload_labels)
+                  BF16, F32, LOSS_SOFTMAX_XENT_LOGITS_MEAN, MXFP4, MXFP8, NN, NT, TN, Gpu, GpuTensor, RtError,
+                  upload_labels)
 
 Shape = Tuple[int, ...]
 
@@ -157,10 +158,22 @@ class Param:
 class Var:
     """tape.rs:135-185: a node of the graph and its device value."""
 
-    __slots__ = ("tape", "idx", "value")
+    __slots__ = ("tape", "idx", "value", "_saved8")
 
     def __init__(self, tape: Tape, idx: int, value: GpuTensor):
         self.tape, self.idx, self.value = tape, idx, value
+        self._saved8: Optional[GpuTensor] = None
+
+    def saved8(self) -> GpuTensor:
+        """The value [rows, columns] in 8 bits (MXFP8), converted once: what a
+        node keeps of it for its backward pass instead of the f32 tensor."""
+        if self._saved8 is None:
+            if len(self.shape) != 2:
+                raise ValueError(f"an 8-bit copy needs rank 2, shape {self.shape}")
+            q = self.gpu.empty(self.shape, MXFP8)
+            self.gpu.convert(self.value, q)
+            self._saved8 = q
+        return self._saved8
 
     @property
     def gpu(self) -> Gpu:
@@ -586,7 +599,7 @@ def apply_activation(z: Var, activation) -> Var:
     raise ValueError(f"unknown activation {activation!r}")
 
 
-def dense_node(x: Var, w: Var, b: Var, relu: bool) -> Var:
+def dense_node(x: Var, w: Var, b: Var, relu: bool, checkpoint: bool = False) -> Var:
     """A = φ(X W + 1ₙ b) for φ = relu or linear as ONE tape node: the GEMM
     applies the bias (and ReLU) in its epilogue, whose arithmetic is the
     reference's matmul, add and relu in sequence (acc + b, then max(·, 0)),
@@ -594,29 +607,42 @@ def dense_node(x: Var, w: Var, b: Var, relu: bool) -> Var:
     exactly where Z > 0), dW = Xᵀδ with db = 1ᵀδ summed in the same launch,
     dX = δ Wᵀ — the ReLU VJP and one paired GEMM launch where the node-per-op
     tape takes four, and one forward launch instead of three.  db is summed in the GEMM's order, not
-    reduce_to's row order: equal within rounding, not bit for bit."""
+    reduce_to's row order: equal within rounding, not bit for bit.
+
+    With ``checkpoint`` the node keeps X, and A for the ReLU mask, in 8 bits
+    (``Var.saved8``, 1.03 bytes an element) instead of f32; the forward values,
+    the mask, db and dX are those of the f32 node, and dW = X₈ᵀδ is exact for
+    the values X₈ that the 8 bits hold, each within 1/16 of X's (or half a step
+    of its block of 32)."""
     gpu = x.gpu
     xv, wv, bv = x.value, w.value, b.value
     (m, k), (k2, n) = xv.shape, wv.shape
     if k != k2 or bv.shape not in ((1, n), (n,)):
         raise ValueError(f"dense: {xv.shape} x {wv.shape} + {bv.shape}")
+    if x.tape is not w.tape or w.tape is not b.tape:
+        raise ValueError("operands belong to different tapes")
     a = gpu.empty((m, n))
     gpu.gemm(NN, xv, wv, a, EPI_BIAS_RELU if relu else EPI_BIAS, bv)
+    out = Var(x.tape, -1, a)
+    kept, mask = xv, a
+    if checkpoint:
+        kept, mask = x.saved8(), out.saved8() if relu else None
 
     def bw(g):
         if relu:
             d = gpu.empty((m, n))
-            gpu.map_vjp("relu", g, a, None, d)
+            gpu.map_vjp("relu", g, mask, None, d)
         else:
             d = g
         dx, dw, db = gpu.empty((m, k)), gpu.empty((k, n)), gpu.empty(bv.shape)
-        gpu.linear_backward(xv, d, wv, dx, dw, db)  # TN + colsum and NT, one launch where it can
+        gpu.linear_backward(kept, d, wv, dx, dw, db)  # TN + colsum and NT, one launch where it can
         return dx, dw, db
 
-    if x.tape is not w.tape or w.tape is not b.tape:
-        raise ValueError("operands belong to different tapes")
-    idx = x.tape._push((x.idx, w.idx, b.idx), bw)
-    return Var(x.tape, idx, a)
+    if not relu:
+        mask = None
+    out.idx = x.tape._push((x.idx, w.idx, b.idx), bw)
+    # bw's cells are kept, mask, wv, bv: a checkpointed node holds no f32 activation.
+    return out
 
 
 class Dense:
@@ -627,11 +653,14 @@ class Dense:
     that follows rtensor's Rng; or pass ``weights`` / ``bias`` directly.
     With ``fused`` (the default) a ReLU or linear layer is one tape node
     (``dense_node``); ``fused=False`` records matmul, add and the activation
-    as the reference does."""
+    as the reference does.  ``checkpoint=True`` keeps the layer's input (and a
+    ReLU's mask) in 8 bits until the backward pass; it needs ``fused``."""
 
     def __init__(self, gpu: Gpu, inputs: int, units: int, activation="linear", rng=None,
-                 weights=None, bias=None, fused: bool = True):
-        self.fused = fused
+                 weights=None, bias=None, fused: bool = True, checkpoint: bool = False):
+        if checkpoint and not fused:
+            raise ValueError("checkpoint needs the fused node")
+        self.fused, self.checkpoint = fused, checkpoint
         if weights is None:
             if rng is None:
                 raise ValueError("Dense needs an rng or explicit weights")
@@ -658,6 +687,11 @@ class Dense:
         t = x.tape
         w, b = self.w.watch(t), self.b.watch(t)
         kind, _ = _activation(self.activation)
+        if self.checkpoint:
+            if len(x.shape) != 2:
+                raise ValueError(f"a checkpointed layer needs rank 2, shape {x.shape}")
+            z = dense_node(x, w, b, kind == "relu", True)
+            return z if kind == "relu" else apply_activation(z, self.activation)
         if self.fused and kind in ("relu", "linear") and len(x.shape) == 2:
             return dense_node(x, w, b, kind == "relu")
         z = x.matmul(w).add(b)
@@ -704,6 +738,47 @@ class Sequential:
         return "\n".join(lines)
 
 
+class QuantizedSequential:
+    """A trained Sequential for inference with its weights in 4 bits: each W is
+    laid out once (``convert_t`` into MXFP4); a layer converts its input to
+    ``activations`` (MXFP8, or MXFP4) and multiplies on the scaled matrix units,
+    bias and ReLU in the epilogue.  Between ReLU and linear layers activations
+    are bf16; the other activation functions, and the result, are f32.  The
+    model's later changes do not reach it."""
+
+    def __init__(self, model: Sequential, activations: int = MXFP8):
+        if activations not in (MXFP4, MXFP8):
+            raise ValueError("activations are MXFP4 or MXFP8")
+        self.activations = activations
+        self.layers = []
+        for layer in model.layers:
+            gpu, (k, n) = layer.w.gpu, layer.w.shape
+            w4 = gpu.empty((n, k), MXFP4)
+            gpu.convert_t(layer.w.tensor, w4)
+            b = gpu.empty((1, n))
+            gpu.map("scale", layer.b.tensor, b, 1.0)
+            self.layers.append((w4, b, layer.activation))
+
+    def predict(self, x) -> GpuTensor:
+        """x [rows, inputs] (f32, bf16 or f16 on the device, or a host array) to f32 [rows, units]."""
+        gpu = self.layers[0][0].gpu
+        x = _as_device(gpu, x)
+        for i, (w4, b, activation) in enumerate(self.layers):
+            kind, slope = _activation(activation)
+            m, (n, k) = x.shape[0], w4.shape
+            if len(x.shape) != 2 or x.shape[1] != k:
+                raise ValueError(f"layer {i} takes [rows, {k}], got {x.shape}")
+            q = gpu.empty((m, k), self.activations)
+            gpu.convert(x, q)
+            fused = kind in ("relu", "linear")
+            y = gpu.empty((m, n), BF16 if fused and i + 1 < len(self.layers) else F32)
+            gpu.gemm(NT, q, w4, y, EPI_BIAS_RELU if kind == "relu" else EPI_BIAS, b)
+            if not fused:
+                gpu.map(kind, y, y, slope)
+            x = y
+        return x
+
+
 __all__ = ["Tape", "constant", "Param", "Var", "Grads", "mse", "mae", "softmax_cross_entropy",
-           "binary_cross_entropy", "one_hot", "accuracy", "Sgd", "Adam", "Dense", "Sequential",
+           "binary_cross_entropy", "one_hot", "accuracy", "Sgd", "Adam", "Dense", "Sequential", "QuantizedSequential",
            "apply_activation", "broadcast_shapes", "RtError"]
