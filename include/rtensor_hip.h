@@ -148,7 +148,21 @@ int rt_convert_t(rt_ctx* ctx, const rt_buf* src, rt_buf* dst);
  * NULL, receives f32 column sums of B over K (= 1ᵀ·B, the bias gradient when
  * B is δ): supported for RT_TN.  Products of f32 have f32 accuracy over the
  * whole range, subnormal operands included, whichever matrix units they run on;
- * infinities and NaN propagate as in f32 arithmetic. */
+ * infinities and NaN propagate as in f32 arithmetic.
+ *
+ * With microscaled operands (no counterpart in the reference):
+ *   - RT_NT, B RT_MXFP4 [N, K], A RT_MXFP4 or RT_MXFP8 [M, K], C f32 or bf16, no
+ *     epilogue, RT_EPI_BIAS or RT_EPI_BIAS_RELU, K <= 2^22: the values of the
+ *     codes are multiplied and added in f32.  With an 8-bit A and a bf16 C a
+ *     product may lose up to 2^-13 of the largest of the eight that share its
+ *     columns 8 j .. 8 j + 7, of whose factors the 8-bit one was rounded by up to
+ *     2^-5 when it was converted.
+ *   - RT_TN, A RT_MXFP8 [K, M], B f32, bf16 or f16 [K, N], C f32, no epilogue,
+ *     with or without colsum, M and N <= 2^22: the weight gradient from an input
+ *     that was saved in 8 bits.  Products are exact (of an f32 B its bits below
+ *     2^-133 are dropped), additions f32.
+ *   - aux of RT_EPI_RELU_MASK may be RT_MXFP8 [M, N] where A and B are f32, bf16
+ *     or f16: 1[x > 0] of the finite values x that were converted into it. */
 int rt_gemm(rt_ctx* ctx, rt_layout layout, const rt_buf* a, const rt_buf* b, rt_buf* c,
             rt_epilogue epi, const rt_buf* aux, rt_buf* colsum);
 

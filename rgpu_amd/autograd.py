@@ -611,9 +611,9 @@ def dense_node(x: Var, w: Var, b: Var, relu: bool, checkpoint: bool = False) -> 
 
     With ``checkpoint`` the node keeps X, and A for the ReLU mask, in 8 bits
     (``Var.saved8``, 1.03 bytes an element) instead of f32; the forward values,
-    the mask, db and dX are those of the f32 node, and dW = X₈ᵀδ is exact for
-    the values X₈ that the 8 bits hold, each within 1/16 of X's (or half a step
-    of its block of 32)."""
+    the mask of finite values, db and dX are those of the f32 node, and
+    dW = X₈ᵀδ is exact for the values X₈ that the 8 bits hold, each within 1/16
+    of X's (or half a step of its block of 32)."""
     gpu = x.gpu
     xv, wv, bv = x.value, w.value, b.value
     (m, k), (k2, n) = xv.shape, wv.shape
@@ -749,6 +749,8 @@ class QuantizedSequential:
     def __init__(self, model: Sequential, activations: int = MXFP8):
         if activations not in (MXFP4, MXFP8):
             raise ValueError("activations are MXFP4 or MXFP8")
+        if not model.layers:
+            raise ValueError("the model has no layers")
         self.activations = activations
         self.layers = []
         for layer in model.layers:
@@ -765,9 +767,10 @@ class QuantizedSequential:
         x = _as_device(gpu, x)
         for i, (w4, b, activation) in enumerate(self.layers):
             kind, slope = _activation(activation)
-            m, (n, k) = x.shape[0], w4.shape
+            n, k = w4.shape
             if len(x.shape) != 2 or x.shape[1] != k:
                 raise ValueError(f"layer {i} takes [rows, {k}], got {x.shape}")
+            m = x.shape[0]
             q = gpu.empty((m, k), self.activations)
             gpu.convert(x, q)
             fused = kind in ("relu", "linear")

@@ -17,6 +17,10 @@ __device__ inline void static_for(F&& f) {
   }
 }
 
+// Whether the value that was converted into this RT_MXFP8 code was positive: a
+// positive one that rounded to zero is 0x80, others that did are 0.
+__device__ inline bool mx_positive(unsigned code) { return code == 0x80u || (code >= 1u && code <= 0x7eu); }
+
 // Workgroup barrier for the direct-to-LDS pipelines: this wave's LDS reads
 // are complete (lgkmcnt 0), then s_barrier.  Unlike __syncthreads it does not
 // wait for outstanding global loads (later stages in flight); the asm's

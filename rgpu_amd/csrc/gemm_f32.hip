@@ -42,12 +42,28 @@ struct F32Args {
   int epi;
   const float* bias;
   const float* mask;
+  const unsigned char* mask8;  // instead of mask: RT_MXFP8 codes, rows of mask8_row bytes
+  long long mask8_row;
   float* colsum;  // [N], or [splits, N] partial rows when splits > 1
   int k_per_split;
   long long split_stride;
   int tiles_m, tiles_n, splits;
   int vec_a, vec_b, vec_c;
 };
+
+// The ReLU mask at one element of C, and at four of a row (col % 4 == 0) as
+// values that are positive where it is.
+__device__ inline bool mask_at(const F32Args& p, long long row, int col) {
+  return p.mask8 ? rt_dev::mx_positive(p.mask8[row * p.mask8_row + col]) : p.mask[row * p.ldc + col] > 0.0f;
+}
+__device__ inline f4 mask4(const F32Args& p, long long row, int col) {
+  if (p.mask8 == nullptr) return *reinterpret_cast<const f4*>(p.mask + row * p.ldc + col);
+  const unsigned w = *reinterpret_cast<const unsigned*>(p.mask8 + row * p.mask8_row + col);
+  f4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = rt_dev::mx_positive((w >> (8 * e)) & 0xffu) ? 1.0f : 0.0f;
+  return v;
+}
 
 // Consecutive workgroups go to different XCDs (round robin over 8), each
 // with its own L2.  Renumber so that every XCD gets a contiguous run of
@@ -289,10 +305,9 @@ __device__ void F32Tile<A_KC, B_KC, BN_>::run(const F32Args& p, int bid, int spl
             for (int u = 0; u < TN; ++u) v[u] = fmaxf(v[u], 0.0f);
           }
         } else if (p.epi == RT_EPI_RELU_MASK) {
-          const float* mrow = p.mask + (long long)row * p.ldc;
 #pragma unroll
           for (int u = 0; u < TN; ++u)
-            if (col0 + u < p.N && !(mrow[col0 + u] > 0.0f)) v[u] = 0.0f;
+            if (col0 + u < p.N && !mask_at(p, row, col0 + u)) v[u] = 0.0f;
         }
       }
       float* dst = Cout + (long long)row * p.ldc + col0;
@@ -547,7 +562,7 @@ __device__ __forceinline__ void store_rows(const F32Args& p, const f4 (&acc)[TM]
             if constexpr (EPI == RT_EPI_BIAS_RELU) v[e] = fmaxf(v[e], 0.0f);
           }
         } else if constexpr (EPI == RT_EPI_RELU_MASK) {
-          const f4 mk = *reinterpret_cast<const f4*>(p.mask + row_off + col);
+          const f4 mk = mask4(p, row, col);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (!(mk[e] > 0.0f)) v[e] = 0.0f;
@@ -563,7 +578,7 @@ __device__ __forceinline__ void store_rows(const F32Args& p, const f4 (&acc)[TM]
           x = x + p.bias[col + e];
           if constexpr (EPI == RT_EPI_BIAS_RELU) x = fmaxf(x, 0.0f);
         } else if constexpr (EPI == RT_EPI_RELU_MASK) {
-          if (!(p.mask[row_off + col + e] > 0.0f)) x = 0.0f;
+          if (!mask_at(p, row, col + e)) x = 0.0f;
         }
         C[row_off + col + e] = x;
       }
@@ -1084,8 +1099,7 @@ struct F32RankK {
     if (vec_mask) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        mkv[i] = m0 + r0 + i < p.M ? *reinterpret_cast<const f4*>(p.mask + (long long)(m0 + r0 + i) * p.ldc + col)
-                                   : f4{0, 0, 0, 0};
+        mkv[i] = m0 + r0 + i < p.M ? mask4(p, m0 + r0 + i, col) : f4{0, 0, 0, 0};
     }
     for (int i = tid; i < 64 * K; i += THREADS) {
       const int r = i / K, k = i - r * K;
@@ -1105,7 +1119,6 @@ struct F32RankK {
       if (row >= p.M) break;
       f4 v = acc[i];
       float* c = p.C + (long long)row * p.ldc + col;
-      const float* mk = p.mask + (long long)row * p.ldc + col;
       if (p.vec_c && col + 4 <= p.N) {
         if (p.epi == RT_EPI_BIAS || p.epi == RT_EPI_BIAS_RELU) {
           v += *reinterpret_cast<const f4*>(p.bias + col);
@@ -1122,7 +1135,7 @@ struct F32RankK {
           if (p.epi == RT_EPI_BIAS || p.epi == RT_EPI_BIAS_RELU) {
             x = x + p.bias[col + q];
             if (p.epi == RT_EPI_BIAS_RELU) x = fmaxf(x, 0.0f);
-          } else if (p.epi == RT_EPI_RELU_MASK && !(mk[q] > 0.0f)) {
+          } else if (p.epi == RT_EPI_RELU_MASK && !mask_at(p, row, col + q)) {
             x = 0.0f;
           }
           c[q] = x;
@@ -1545,7 +1558,7 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void gemm_f32_skinny_kernel(F32A
       v = v + p.bias[col];
       if (p.epi == RT_EPI_BIAS_RELU) v = fmaxf(v, 0.0f);
     } else if (p.epi == RT_EPI_RELU_MASK) {
-      if (!(p.mask[(long long)row * p.ldc + col] > 0.0f)) v = 0.0f;
+      if (!mask_at(p, row, col)) v = 0.0f;
     }
     p.C[(long long)row * p.ldc + col] = v;
   }
@@ -1602,6 +1615,7 @@ hipError_t dispatch_tile(hipStream_t s, F32Args a) {
     rest.A += A_KC ? (long long)kMostRows * a.lda : (long long)kMostRows;
     rest.C += (long long)kMostRows * a.ldc;
     if (rest.mask != nullptr) rest.mask += (long long)kMostRows * a.ldc;
+    if (rest.mask8 != nullptr) rest.mask8 += kMostRows * a.mask8_row;
     rest.colsum = nullptr;  // the first part's
     return dispatch_tile<A_KC, B_KC>(s, rest);
   }
@@ -1637,6 +1651,8 @@ F32Args make_args(const rt::GemmDesc& d) {
   a.epi = d.epi;
   a.bias = d.bias;
   a.mask = static_cast<const float*>(d.mask);
+  a.mask8 = d.mask8;
+  a.mask8_row = d.mask8_row;
   a.colsum = d.splits > 1 ? d.colsum_partials : d.colsum;
   a.splits = d.splits < 1 ? 1 : d.splits;
   // Slices are whole multiples of the 32-wide K step.

@@ -61,6 +61,8 @@ struct HalfArgs {
   const float* bias;
   const void* mask;
   int mask_bf16;  // mask dtype: 1 = bf16, 0 = f32
+  const unsigned char* mask8;  // instead of mask: RT_MXFP8 codes, rows of mask8_row bytes
+  long long mask8_row;
   int out_bf16;
   float* colsum;
   float* cs_parts;  // non-null: per-M-tile column-sum shares [splits * tiles_m, N]
@@ -226,6 +228,10 @@ __device__ __forceinline__ void store_tile(const HalfArgs& p, f4 (&acc)[TM][TN],
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if (e < nv) {
+              if (p.mask8) {
+                if (!rt_dev::mx_positive(p.mask8[row * p.mask8_row + col + e])) v[e] = 0.0f;
+                continue;
+              }
               const float mv = p.mask_bf16 ? bf16_to_f32(static_cast<const unsigned short*>(p.mask)[off + e])
                                            : static_cast<const float*>(p.mask)[off + e];
               if (!(mv > 0.0f)) v[e] = 0.0f;
@@ -493,6 +499,16 @@ struct DmaOperand {
   }
 };
 
+// Four columns (col % 4 == 0) of an 8-bit mask, as values that are positive where
+// it is; a row of codes is padded to whole 128 columns.
+__device__ inline f4 mask8_at(const HalfArgs& p, long long row, int col) {
+  const unsigned w = *reinterpret_cast<const unsigned*>(p.mask8 + row * p.mask8_row + col);
+  f4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = rt_dev::mx_positive((w >> (8 * e)) & 0xffu) ? 1.0f : 0.0f;
+  return v;
+}
+
 // Full-tile epilogue straight from the accumulators.  The DMA kernel issues
 // its MFMAs with the operands swapped (D = op(B)·op(A)), so lane (g, r) holds
 // C(m0+wm+16t+r, n0+wn+16u+4g+q) for q = 0..3: four consecutive columns of
@@ -560,7 +576,9 @@ __device__ __forceinline__ void store_direct(const HalfArgs& p, const f4 (&acc)[
             if (!((nib >> e) & 1u)) v[e] = 0.0f;
         } else {
           f4 mk;
-          if (p.mask_bf16) {
+          if (p.mask8) {
+            mk = mask8_at(p, m0 + wm + 16 * t + r, col);
+          } else if (p.mask_bf16) {
             const u2 h = *reinterpret_cast<const u2*>(static_cast<const unsigned short*>(p.mask) + off);
             mk = f4{__uint_as_float(h[0] << 16), __uint_as_float(h[0] & 0xffff0000u), __uint_as_float(h[1] << 16),
                     __uint_as_float(h[1] & 0xffff0000u)};
@@ -670,7 +688,9 @@ __device__ __forceinline__ void store_edge(const HalfArgs& p, const f4 (&acc)[TM
         }
       } else if (epi == RT_EPI_RELU_MASK) {
         f4 mk;
-        if (vec_mask && nv == 4 && p.mask_bf16) {
+        if (p.mask8) {
+          mk = mask8_at(p, row, col);
+        } else if (vec_mask && nv == 4 && p.mask_bf16) {
           const u2 h = *reinterpret_cast<const u2*>(static_cast<const unsigned short*>(p.mask) + off);
           mk = f4{__uint_as_float(h[0] << 16), __uint_as_float(h[0] & 0xffff0000u), __uint_as_float(h[1] << 16),
                   __uint_as_float(h[1] & 0xffff0000u)};
@@ -1183,6 +1203,8 @@ static HalfArgs half_args(const GemmDesc& d, int splits) {
   a.bias = d.bias;
   a.mask = d.mask;
   a.mask_bf16 = d.mask_dtype == RT_BF16;
+  a.mask8 = d.mask8;
+  a.mask8_row = d.mask8_row;
   a.out_bf16 = splits == 1 && d.out_dtype == RT_BF16;
   a.colsum = splits > 1 ? d.colsum_partials : d.colsum;
   int kps = (d.K + splits - 1) / splits;

@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "device_util.h"
 #include "mx_device.h"
 #include "rt_internal.h"
 
@@ -107,10 +108,10 @@ template <typename T, bool FP4>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ src, long long rows, long long cols,
                                                        unsigned char* __restrict__ codes,
                                                        unsigned char* __restrict__ scales, long long steps,
-                                                       long long groups) {
+                                                       long long groups, long long block0) {
   constexpr int V = 16 / sizeof(T), LANES = 128 / V, ROWS = 256 / LANES, PASSES = 64 / ROWS;
   __shared__ unsigned sc[64];
-  const long long step = blockIdx.x % steps, group = blockIdx.x / steps;
+  const long long block = block0 + blockIdx.x, step = block % steps, group = block / steps;
   const int lane = threadIdx.x % LANES, row0 = threadIdx.x / LANES;
   const long long col = step * 128 + lane * V;
   if (threadIdx.x < 64) sc[threadIdx.x] = 0;
@@ -166,11 +167,12 @@ template <typename T, bool FP4>
 __global__ __launch_bounds__(256) void quantize_t_kernel(const T* __restrict__ src, long long rows, long long cols,
                                                          unsigned char* __restrict__ codes,
                                                          unsigned char* __restrict__ scales, long long steps,
-                                                         long long groups) {
+                                                         long long groups, long long block0) {
   constexpr int W = 4 / sizeof(T);
   typedef unsigned int any_u1 __attribute__((aligned(2)));
   __shared__ unsigned sc[64 * W];
-  const long long blocks = (groups + W - 1) / W, group = blockIdx.x % blocks * W, step = blockIdx.x / blocks;
+  const long long block = block0 + blockIdx.x, blocks = (groups + W - 1) / W;
+  const long long group = block % blocks * W, step = block / blocks;
   const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
   const long long row = group * 64 + W * lane, col = step * 128 + 32 * g;
   if (threadIdx.x < 64 * W) sc[threadIdx.x] = 0;
@@ -250,10 +252,10 @@ template <typename T, bool FP4>
 __global__ __launch_bounds__(256) void dequantize_kernel(const unsigned char* __restrict__ codes,
                                                          const unsigned char* __restrict__ scales, T* __restrict__ dst,
                                                          long long rows, long long cols, long long steps,
-                                                         long long groups) {
+                                                         long long groups, long long block0) {
   constexpr int V = 16 / sizeof(T), LANES = 128 / V, ROWS = 256 / LANES, PASSES = 64 / ROWS;
   __shared__ unsigned sc[64];
-  const long long step = blockIdx.x % steps, group = blockIdx.x / steps;
+  const long long block = block0 + blockIdx.x, step = block % steps, group = block / steps;
   const int lane = threadIdx.x % LANES, row0 = threadIdx.x / LANES;
   const long long col = step * 128 + lane * V, row_bytes = steps * (FP4 ? 64 : 128);
   if (threadIdx.x < 64)
@@ -298,62 +300,61 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const unsigned char* __
   }
 }
 
-// Whether the value converted into this 8-bit code was positive (rt_convert's rule).
-__device__ inline bool positive(unsigned code) { return code == 0x80u || (code >= 1u && code <= 0x7eu); }
-
 // v zeroed where the mask is not positive (VJP false), or v = g · 1[mask > 0]
-// as a product (VJP true: f32).  A thread takes 16 bytes of v in a row, read,
-// masked and written whole where the row has room (single elements written as
-// zeros took twice as long: 2048 x 1024 f32 5.8 us).
-template <typename T, bool VJP>
+// as a product (VJP true).  A thread takes four values of a row, read, masked and
+// written whole where the row has room.
+template <bool VJP>
 __global__ __launch_bounds__(256) void mask_kernel(const unsigned char* __restrict__ codes, unsigned rows,
-                                                   unsigned cols, long long row_bytes, const T* g, T* v) {
-  constexpr int V = 16 / sizeof(T);
-  const unsigned chunks = (cols + V - 1) / V;
-  const unsigned per_block = gridDim.x;  // blocks along a row; blockIdx.y: rows
+                                                   unsigned cols, long long row_bytes, const float* g, float* v) {
+  const unsigned chunks = (cols + 3) / 4;
   for (unsigned row = blockIdx.y * blockDim.y + threadIdx.y; row < rows; row += gridDim.y * blockDim.y)
-    for (unsigned c = blockIdx.x * blockDim.x + threadIdx.x; c < chunks; c += per_block * blockDim.x) {
-      const unsigned col = c * V;
-      unsigned w[V / 4];
-      __builtin_memcpy(w, __builtin_assume_aligned(codes + row * row_bytes + col, V), V);
-      T* at = v + (long long)row * cols + col;
-      const T* from = VJP ? g + (long long)row * cols + col : at;
-      const int n = min((unsigned)V, cols - col);
-      T x[V];
-      if (n == V) {
+    for (unsigned c = blockIdx.x * blockDim.x + threadIdx.x; c < chunks; c += gridDim.x * blockDim.x) {
+      const unsigned col = 4 * c, w = *reinterpret_cast<const unsigned*>(codes + row * row_bytes + col);
+      float* at = v + (long long)row * cols + col;
+      const float* from = VJP ? g + (long long)row * cols + col : at;
+      const int n = min(4u, cols - col);
+      float x[4];
+      if (n == 4) {
         __builtin_memcpy(x, from, sizeof x);
       } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = e < n ? from[e] : Elem<T>::put(0.0f);
+        for (int e = 0; e < 4; ++e) x[e] = e < n ? from[e] : 0.0f;
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const bool on = positive((w[e / 4] >> (8 * (e % 4))) & 0xffu);
+      for (int e = 0; e < 4; ++e) {
+        const bool on = rt_dev::mx_positive((w >> (8 * e)) & 0xffu);
         if constexpr (VJP) x[e] = x[e] * (on ? 1.0f : 0.0f);
-        else x[e] = on ? x[e] : Elem<T>::put(0.0f);
+        else x[e] = on ? x[e] : 0.0f;
       }
-      if (n == V) {
+      if (n == 4) {
         __builtin_memcpy(at, x, sizeof x);
       } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e)
+        for (int e = 0; e < 4; ++e)
           if (e < n) at[e] = x[e];
       }
     }
 }
 
-template <typename T, bool VJP>
-hipError_t mask(hipStream_t s, const rt::MxTensor& m, const T* g, T* v) {
+template <bool VJP>
+hipError_t mask(hipStream_t s, const rt::MxTensor& m, const float* g, float* v) {
   if (m.rows == 0 || m.cols == 0) return hipSuccess;
-  const unsigned chunks = (unsigned)((m.cols + 16 / (int)sizeof(T) - 1) / (16 / (int)sizeof(T)));
+  const unsigned chunks = (unsigned)((m.cols + 3) / 4);
   // A block: 256 threads over a row, or over several short ones.
   unsigned bx = 256;
   while (bx > 16 && bx / 2 >= chunks) bx /= 2;
   const unsigned by = 256 / bx, gx = std::min((chunks + bx - 1) / bx, 4096u);
   const unsigned gy = (unsigned)std::min<long long>((m.rows + by - 1) / by, std::max(1u, 32768u / gx));
-  rt::launch((mask_kernel<T, VJP>), dim3(gx, gy), dim3(bx, by), 0, s, m.codes, (unsigned)m.rows, (unsigned)m.cols,
+  rt::launch(mask_kernel<VJP>, dim3(gx, gy), dim3(bx, by), 0, s, m.codes, (unsigned)m.rows, (unsigned)m.cols,
              (long long)rt::mx_layout(m.dtype, m.rows, m.cols).row_bytes, g, v);
   return hipGetLastError();
+}
+
+// A grid holds fewer than 2^32 threads: more blocks go in several launches.
+template <typename F>
+void in_launches(long long blocks, F&& launch) {
+  constexpr long long kMost = 1LL << 23;
+  for (long long b = 0; b < blocks; b += kMost) launch(b, (unsigned)std::min(kMost, blocks - b));
 }
 
 template <typename T>
@@ -363,8 +364,10 @@ hipError_t quantize(hipStream_t s, const void* src, bool transposed, const rt::M
   auto* scales = const_cast<unsigned char*>(d.scales);
   const size_t per = transposed ? 4 / sizeof(T) : 1;  // groups a block
   auto go = [&](auto kernel) {
-    rt::launch(kernel, dim3((unsigned)(l.steps * ((l.groups + per - 1) / per))), dim3(256), 0, s,
-               static_cast<const T*>(src), d.rows, d.cols, codes, scales, (long long)l.steps, (long long)l.groups);
+    in_launches((long long)(l.steps * ((l.groups + per - 1) / per)), [&](long long block0, unsigned n) {
+      rt::launch(kernel, dim3(n), dim3(256), 0, s, static_cast<const T*>(src), d.rows, d.cols, codes, scales,
+                 (long long)l.steps, (long long)l.groups, block0);
+    });
   };
   if (d.dtype == RT_MXFP4) transposed ? go(quantize_t_kernel<T, true>) : go(quantize_kernel<T, true>);
   else transposed ? go(quantize_t_kernel<T, false>) : go(quantize_kernel<T, false>);
@@ -375,8 +378,10 @@ template <typename T>
 hipError_t dequantize(hipStream_t s, const rt::MxTensor& m, void* dst) {
   const rt::MxLayout l = rt::mx_layout(m.dtype, m.rows, m.cols);
   auto go = [&](auto kernel) {
-    rt::launch(kernel, dim3((unsigned)(l.steps * l.groups)), dim3(256), 0, s, m.codes, m.scales, static_cast<T*>(dst),
-               m.rows, m.cols, (long long)l.steps, (long long)l.groups);
+    in_launches((long long)(l.steps * l.groups), [&](long long block0, unsigned n) {
+      rt::launch(kernel, dim3(n), dim3(256), 0, s, m.codes, m.scales, static_cast<T*>(dst), m.rows, m.cols,
+                 (long long)l.steps, (long long)l.groups, block0);
+    });
   };
   m.dtype == RT_MXFP4 ? go(dequantize_kernel<T, true>) : go(dequantize_kernel<T, false>);
   return hipGetLastError();
@@ -416,14 +421,10 @@ hipError_t mx_dequantize_launch(hipStream_t s, const MxTensor& src, void* dst, i
   return hipErrorInvalidValue;
 }
 
-hipError_t mx_mask_launch(hipStream_t s, const MxTensor& m, void* v, int v_dtype) {
-  if (v_dtype == RT_F32) return mask<float, false>(s, m, nullptr, static_cast<float*>(v));
-  if (v_dtype == RT_BF16) return mask<bf16_bits, false>(s, m, nullptr, static_cast<bf16_bits*>(v));
-  return hipErrorInvalidValue;
-}
+hipError_t mx_mask_launch(hipStream_t s, const MxTensor& m, float* v) { return mask<false>(s, m, nullptr, v); }
 
 hipError_t mx_relu_vjp_launch(hipStream_t s, const MxTensor& m, const float* g, float* dx) {
-  return mask<float, true>(s, m, g, dx);
+  return mask<true>(s, m, g, dx);
 }
 
 }  // namespace rt

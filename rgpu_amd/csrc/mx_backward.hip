@@ -670,8 +670,8 @@ struct Plan {
 // tiles unsplit 32.6, 3 slices 23.9, 8 30; 128 tiles 4 slices 25.8, unsplit 41.8;
 // f32: 64 tiles 4 slices 33.2, unsplit 62.3.  600 rows, 2000 x 1500, bf16: 64
 // tiles 17.9 unsplit, 29 in 2 slices.  5000 rows, 200 x 64, bf16: 64 tiles 69
-// unsplit, 9.9 in 32 slices.  8192 rows, 4096 x 4096, bf16: 239 with 256 tiles,
-// 355 with 128.
+// unsplit, 9.9 in 32 slices.  8192 rows, 4096 x 4096, bf16: 256 with 256 tiles,
+// 399 with 128.
 Plan plan(const rt::MxTensor& x, const void* delta, int dtype, long long N) {
   struct Tile {
     int size;

@@ -458,9 +458,9 @@ hipError_t launch_tiles(hipStream_t s, Args p) {
 
 // Tiles by what fills the chip.  256 x 256 (4 bits) has a CU to itself, so it
 // takes whole rounds of 256, or a last one that leaves no more than a third of
-// all places idle (K 4096, us with 256 and 128 tiles: 8192 x 4096, 512 blocks, 80
-// and 93; 6912 x 4864, 513 blocks, 104 and 110; 4608 x 4096, 288 blocks, 66 and
-// 56).  128 x 128, two a CU, from 208 blocks on (1800 x 1800, K 2000, 225 blocks,
+// all places idle (us with 256 and 128 tiles: 4096 x 4096, K 1024, 256 blocks,
+// 19.0 and 21.1; K 4096: 6912 x 4864, 513 blocks, 104 and 110; 4608 x 4096, 288
+// blocks, 66 and 56).  128 x 128, two a CU, from 208 blocks on (1800 x 1800, K 2000, 225 blocks,
 // 8 bits: 13.2 and 13.9 with 64 tiles; 700 x 4096, K 1000, 192 blocks: 12.0 and
 // 10.6).  For 8 bits larger tiles were no faster (256 x 128, 8192 x 4096, K 4096:
 // 119.7 and 115.9 with 128).
@@ -481,7 +481,8 @@ hipError_t launch_many(hipStream_t s, const Args& p) {
 // K 1024 5.4 and 5.7).
 template <int ABITS>
 hipError_t launch(hipStream_t s, const Args& p) {
-  if (p.M <= 48 || (p.M <= 64 && p.steps <= 8)) {
+  // (A grid holds fewer than 2^32 threads.)
+  if ((p.M <= 48 || (p.M <= 64 && p.steps <= 8)) && p.N <= (1 << 26)) {
     const dim3 grid((unsigned)((p.N + 15) / 16)), block(64 * kRowWaves);
     const int tm = (p.M + 15) / 16;
     if (tm == 1) rt::launch(mx_rows_kernel<ABITS, 1>, grid, block, 0, s, p);

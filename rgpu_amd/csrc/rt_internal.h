@@ -181,6 +181,10 @@ struct GemmDesc {
   const float* bias = nullptr;    // [N] f32
   const void* mask = nullptr;     // [M, N], ld = ldc, dtype = mask_dtype
   int mask_dtype = RT_F32;
+  // Instead of mask: the codes of an RT_MXFP8 mask and a row's bytes (unsplit
+  // launches).
+  const unsigned char* mask8 = nullptr;
+  long long mask8_row = 0;
   float* colsum = nullptr;        // [N] f32 = 1ᵀ·B over this launch's K range
   int splits = 1;                 // K slices (blockIdx.z); >1 writes f32 partial planes
   long long split_stride = 0;     // elements between partial planes of C
@@ -292,8 +296,8 @@ MxTensor mx_tensor(const rt_buf* b);
 // src f32/bf16/f16 [rows, cols] -> dst, or with transposed [cols, rows] -> dst [rows, cols].
 hipError_t mx_quantize_launch(hipStream_t s, const void* src, int src_dtype, bool transposed, const MxTensor& dst);
 hipError_t mx_dequantize_launch(hipStream_t s, const MxTensor& src, void* dst, int dst_dtype);
-// v (f32 or bf16, the mask's shape) zeroed where the mask is not positive.
-hipError_t mx_mask_launch(hipStream_t s, const MxTensor& mask, void* v, int v_dtype);
+// v (the mask's shape) zeroed where the mask is not positive.
+hipError_t mx_mask_launch(hipStream_t s, const MxTensor& mask, float* v);
 // dx = g · 1[mask > 0], as a product (the VJP of the tape's ReLU).
 hipError_t mx_relu_vjp_launch(hipStream_t s, const MxTensor& mask, const float* g, float* dx);
 // C [M, N] = A·Bᵀ with A [M, K] and B RT_MXFP4 [N, K]; epi none, bias or bias and ReLU.

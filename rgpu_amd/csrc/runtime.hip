@@ -592,13 +592,6 @@ int rt_gemm(rt_ctx* c, rt_layout layout, const rt_buf* a, const rt_buf* b, rt_bu
     if (colsum->dtype != RT_F32 || colsum->n != N) return fail(c, RT_ERR_SHAPE, "colsum must be f32 [%zu]", N);
   }
   if (M == 0 || N == 0) return RT_OK;
-  if (epi == RT_EPI_RELU_MASK && aux->dtype == RT_MXFP8) {
-    // The product as it stands, then the mask.
-    if ((rc = rt_gemm(c, layout, a, b, out, RT_EPI_NONE, nullptr, colsum))) return rc;
-    Launch L(c, "mx_mask");
-    HIP_TRY(c, mx_mask_launch(c->stream, mx_tensor(aux), out->ptr, out->dtype), "mask");
-    return RT_OK;
-  }
   GemmDesc d;
   d.layout = layout;
   d.in_dtype = a->dtype;
@@ -614,7 +607,10 @@ int rt_gemm(rt_ctx* c, rt_layout layout, const rt_buf* a, const rt_buf* b, rt_bu
   d.ldc = (int)N;
   d.epi = epi;
   if (epi == RT_EPI_BIAS || epi == RT_EPI_BIAS_RELU) d.bias = static_cast<const float*>(aux->ptr);
-  if (epi == RT_EPI_RELU_MASK) {
+  if (epi == RT_EPI_RELU_MASK && aux->dtype == RT_MXFP8) {
+    d.mask8 = static_cast<const unsigned char*>(aux->ptr);
+    d.mask8_row = (long long)mx_layout(RT_MXFP8, M, N).row_bytes;
+  } else if (epi == RT_EPI_RELU_MASK) {
     d.mask = aux->ptr;
     d.mask_dtype = aux->dtype;
   }
@@ -854,7 +850,7 @@ int rt_relu_bwd(rt_ctx* c, const rt_buf* a, rt_buf* delta) {
   if (a->n == 0) return RT_OK;
   Launch L(c, "relu_bwd");
   if (a->dtype == RT_MXFP8) {
-    HIP_TRY(c, mx_mask_launch(c->stream, mx_tensor(a), delta->ptr, RT_F32), "relu_bwd");
+    HIP_TRY(c, mx_mask_launch(c->stream, mx_tensor(a), static_cast<float*>(delta->ptr)), "relu_bwd");
     return RT_OK;
   }
   HIP_TRY(c, relu_bwd_launch(c->stream, a->ptr, a->dtype, static_cast<float*>(delta->ptr), a->n), "relu_bwd");

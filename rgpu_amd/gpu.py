@@ -352,6 +352,8 @@ class Gpu:
         ``shape`` as ``download`` gives them."""
         a = np.asarray(a)
         if dtype in (MXFP4, MXFP8):
+            if shape is None:
+                raise ValueError("the bytes of a microscaled tensor need its shape")
             host, shape = np.ascontiguousarray(a, dtype=np.uint8), _shape(shape)
             if host.nbytes != tensor_bytes(shape, dtype):
                 raise ValueError(f"a tensor {shape} has {tensor_bytes(shape, dtype)} bytes, got {host.nbytes}")

@@ -110,6 +110,8 @@ def test_refusals(gpu):
     assert status(gpu.sum_all, m8, f()) == "RT_ERR_DTYPE"
     with pytest.raises(ValueError):
         gpu.upload(np.zeros(5, np.uint8), G.MXFP4, (8, 40))
+    with pytest.raises(ValueError):
+        gpu.upload(np.zeros(5, np.uint8), G.MXFP4)
     gpu.sync()
 
 
@@ -379,6 +381,35 @@ def test_dw_f16_scales_beyond_f16(gpu, rows, N):
     check_dw(gpu, rows, 300, N, "f16", x=x)
 
 
+def test_dw_f16_scales_beyond_f16_in_large_tiles(gpu):
+    # whole 256 x 256 tiles, some of which take the other way
+    rng = np.random.default_rng(12)
+    x = rng.normal(size=(300, 4100)).astype(np.float32)
+    x[:, 600:610] *= np.float32(2.0 ** 20)
+    check_dw(gpu, 300, 4100, 4096, "f16", x=x)
+
+
+@pytest.mark.parametrize("rows,K,N", [(100, 60, 50), (300, 2000, 2048)])
+def test_dw_subnormal_values(gpu, rows, K, N):
+    """Halves down to their last bit; f32 down to 2^-133, the last bit of a bf16; 8-bit values far below f16's range."""
+    rng = np.random.default_rng(13)
+    x = (rng.normal(size=(rows, K)) * 2.0 ** 20).astype(np.float32)
+    q, xv = mx_upload(gpu, x, G.MXFP8)
+    dw = gpu.empty((K, N))
+    for dtype, scale in (("f16", 2.0 ** -22), ("bf16", 2.0 ** -128), ("f32", 2.0 ** -128)):
+        d64 = rounded(rng.normal(size=(rows, N)) * scale, DTYPE[dtype])
+        gpu.matmul_at_b(q, gpu.upload(d64, DTYPE[dtype]), dw)
+        size = np.abs(xv).T @ np.abs(d64)
+        lost = 2.0 ** -133 * np.abs(xv).sum(0)[:, None] if dtype == "f32" else 0
+        assert np.all(np.abs(gpu.download(dw) - xv.T @ d64) <= (3 * rows + 40) * 2.0 ** -23 * size + lost)
+    small = (rng.normal(size=(rows, K)) * 2.0 ** -60).astype(np.float32)
+    q, xv = mx_upload(gpu, small, G.MXFP8)
+    for dtype in DTYPE:
+        d64 = rounded(rng.normal(size=(rows, N)), DTYPE[dtype])
+        gpu.matmul_at_b(q, gpu.upload(d64, DTYPE[dtype]), dw)
+        assert np.all(np.abs(gpu.download(dw) - xv.T @ d64) <= (3 * rows + 40) * 2.0 ** -23 * (np.abs(xv).T @ np.abs(d64)))
+
+
 @pytest.mark.parametrize("dtype", sorted(DTYPE))
 @pytest.mark.parametrize("N", [1, 7, 63, 129])
 def test_dw_from_any_place_in_memory(gpu, dtype, N):
@@ -456,13 +487,35 @@ def test_masks_are_exact(gpu, rows, cols):
     dx = gpu.empty((rows, cols))
     gpu.map_vjp("relu", gpu.upload(g), q, None, dx)
     assert np.array_equal(gpu.download(dx), g * on)
-    # the mask of a product is that of the separate pass
-    for dtype, out in ((G.F32, G.F32), (G.BF16, G.BF16), (G.BF16, G.F32), (G.F16, G.F32)):
-        a, w = gpu.upload(rng.normal(size=(rows, 40)), dtype), gpu.upload(rng.normal(size=(cols, 40)), dtype)
-        plain, masked = gpu.empty((rows, cols), out), gpu.empty((rows, cols), out)
-        gpu.matmul_a_bt(a, w, plain)
-        gpu.matmul_a_bt(a, w, masked, relu_mask_from=q)
-        assert np.array_equal(gpu.download_f32(masked), np.where(on, gpu.download_f32(plain), 0))
+
+
+@pytest.mark.parametrize("rows,cols,K", [(1, 1, 8), (3, 5, 40), (37, 130, 300), (200, 1003, 7), (40, 64, 256), (64, 128, 64),
+                                         (128, 256, 512), (130, 260, 200), (2048, 1024, 128), (1030, 2056, 264),
+                                         (4096, 4096, 64)])
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f32"), ("f16", "bf16")])
+def test_mask_of_a_product(gpu, rows, cols, K, dtype, out):
+    """The masked product is the plain one with zeros, whichever kernel the sizes go to (rows of a few, of whole tiles, of
+    none), also where the plain one is not a number."""
+    rng = np.random.default_rng(rows + cols)
+    x = X.values(rng, rows, cols)
+    q = gpu.zeros((rows, cols), G.MXFP8)
+    gpu.convert(gpu.upload(x), q)
+    a, w = rng.normal(size=(rows, K)), rng.normal(size=(cols, K))
+    a[rows // 2, 0] = np.nan
+    ga, gw = gpu.upload(a, DTYPE[dtype]), gpu.upload(w, DTYPE[dtype])
+    plain, masked = gpu.empty((rows, cols), DTYPE[out]), gpu.empty((rows, cols), DTYPE[out])
+    gpu.matmul_a_bt(ga, gw, plain)
+    gpu.matmul_a_bt(ga, gw, masked, relu_mask_from=q)
+    assert np.array_equal(gpu.download_f32(masked), np.where(x > 0, gpu.download_f32(plain), 0), equal_nan=True)
+    if rows * cols < 10000:  # the other layouts
+        for layout, (sa, sb) in ((G.NN, (a, w.T)), (G.TN, (a.T, w.T))):
+            u, v = gpu.upload(np.ascontiguousarray(sa), DTYPE[dtype]), gpu.upload(np.ascontiguousarray(sb), DTYPE[dtype])
+            gpu.gemm(layout, u, v, plain)
+            gpu.gemm(layout, u, v, masked, G.EPI_RELU_MASK, q)
+            want, got = np.where(x > 0, gpu.download_f32(plain), 0).astype(np.float64), gpu.download_f32(masked)
+            assert np.array_equal(np.isnan(want), np.isnan(got)) and not got[x <= 0].any()
+            size = np.abs(np.nan_to_num(a)) @ np.abs(w).T
+            assert np.all(np.abs(np.nan_to_num(got - want)) <= (K + 8) * 2.0 ** -22 * size + 2.0 ** -7 * np.abs(np.nan_to_num(want)))
 
 
 @pytest.mark.parametrize("dtype", sorted(DTYPE))

@@ -187,7 +187,11 @@ def test_quantized_model_is_its_operators_in_a_row(gpu, rows, activations):
     with pytest.raises(ValueError):
         served.predict(np.zeros((rows, 99), np.float32))
     with pytest.raises(ValueError):
+        served.predict(np.float32(1.0))
+    with pytest.raises(ValueError):
         A.QuantizedSequential(model, G.F32)
+    with pytest.raises(ValueError):
+        A.QuantizedSequential(A.Sequential([]))
     # the served weights are a copy
     model.layers[0].w.set(np.zeros((100, 130), np.float32))
     model.layers[0].b.set(np.zeros((1, 130), np.float32))
