@@ -4,12 +4,13 @@
 //
 // A value of X has four significant bits and a power of two, so it is a bf16
 // without rounding, and an f16 too where its block's scale is from 2^-15 to 2^7.
-// bf16 δ is multiplied as it stands; f16 δ as well where the block's part of X
-// has only such scales (a block looks its scales over first: 1/32 of its codes'
-// bytes; 262144 rows of 512 x 512 160 us, 408 in planes), else as two bf16
-// planes (11 bits); f32 δ as three (24 bits, each plane the next eight by
-// truncation).  So every product is exact, and the sums are
-// f32.  The scale of X varies along the rows that are summed, so it cannot stay
+// bf16 δ is multiplied as it stands; f16 δ as well where the scales of the
+// workgroup's part of X span no more than those 22 powers of two: X is multiplied
+// by a power of two that brings them there, C by its inverse (a workgroup looks
+// its scales over first: 1/32 of its codes' bytes).  Else f16 δ goes in as two
+// bf16 planes (11 bits; 262144 rows of 512 x 512 521 us, 160 as it stands); f32 δ
+// as three (24 bits, each plane the next eight by truncation).  So every product
+// is exact, and the sums are f32.  The scale of X varies along the rows that are summed, so it cannot stay
 // outside the product: X is decoded on its way into LDS, where a thread holds 16
 // columns of one row, which share a scale.
 //
@@ -61,6 +62,7 @@ struct Args {
 struct Place {
   int slice, tile_m, m0, n0;
   long long rb, re;  // its rows of X and δ
+  int shift;         // X is multiplied by 2^shift, C by 2^-shift (f16)
 };
 template <int BM, int BN>
 __device__ inline Place place(const Args& p) {
@@ -78,6 +80,7 @@ __device__ inline Place place(const Args& p) {
   q.n0 = (in_band / size) * BN;
   q.rb = q.slice * p.rows_per_split;
   q.re = min(p.rows, q.rb + p.rows_per_split);
+  q.shift = 0;
   return q;
 }
 
@@ -137,6 +140,7 @@ struct XSide {
   };
   Cursor codes, scales;
   int k, voff, svoff, vstep, rows;  // row and place of the first chunk; rows of the slice
+  int shift;
   __device__ inline void init(const Args& p, const Place& at, int tid) {
     const int c = at.m0 % 128 / 16 + tid % XR;  // chunk of its 128 columns, and beyond
     k = tid / XR;
@@ -144,6 +148,7 @@ struct XSide {
     vstep = 32 * p.x_row;
     svoff = c / 8 * (p.x_groups * 256) + 4 * (16 * (c % 8 / 2) + k % 16);
     rows = (int)(at.re - at.rb);
+    shift = at.shift;
     codes = Cursor{reinterpret_cast<const char*>(p.x + at.rb * p.x_row + at.m0), (long long)rows * p.x_row - at.m0,
                    (long long)ROWS * p.x_row};
     const long long first = (long long)(at.m0 / 128) * p.x_groups + at.rb / 64;
@@ -163,7 +168,8 @@ struct XSide {
   template <bool F16>
   __device__ inline void decode(int s, const Raw& x, int i, u4 (&h)[2]) const {
     const int row = s * ROWS + k + 32 * i;
-    const unsigned byte = (x.scales >> (8 * (row % 64 / 16))) & 0xffu;
+    unsigned byte = (x.scales >> (8 * (row % 64 / 16))) & 0xffu;
+    if constexpr (F16) byte = (unsigned)max((int)byte + shift, 0);
     decode16<F16>(x.w[i], row < rows ? byte : 0u, h);
   }
 };
@@ -182,10 +188,18 @@ __device__ inline f4 mfma(const u4& a, const u4& b, const f4& acc) {
 // C's tile (or its plane of the slice): lane (g, r) holds four consecutive
 // columns of a row.
 template <int TM, int TN>
-__device__ __forceinline__ void store_c(const Args& p, const f4 (&acc)[TM][TN], const Place& at, int wm, int wn, int g,
+__device__ __forceinline__ void store_c(const Args& p, f4 (&acc)[TM][TN], const Place& at, int wm, int wn, int g,
                                         int r) {
   float* c = p.c + at.slice * p.split_stride;
   const bool vec = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(c) & 15) == 0;
+  if (at.shift != 0) {
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+#pragma unroll
+      for (int u = 0; u < TN; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][u][e] = ldexpf(acc[t][u][e], -at.shift);
+  }
   static_for<0, TM>([&](auto tc) {
     constexpr int t = decltype(tc)::value;
     const int row = at.m0 + wm + 16 * t + r;
@@ -612,12 +626,15 @@ __device__ __forceinline__ void direct_body(const Args& p, const Place& at, unsi
   store_c<TM, TN>(p, acc, at, wm, wn, g, r);
 }
 
-// Whether f16 holds the values of the block's part of X: scales from 2^-15 to
-// 2^7 (448·2^7 and 2^-9·2^-15 are f16 values).  A byte of 0 is a block of zeros
-// (or of values below 2^-118, which count as zeros).
+// The shift at which f16 holds the values of the workgroup's part of X: one that
+// puts its scales between 2^-15 and 2^7 (448·2^7 and 2^-9·2^-15 are f16 values), 0
+// where they are; or kNoShift.  A byte of 0 is a block of zeros (or of values up to
+// 2^-118, which are zeros where the shift does not bring them up); 255, NaN, is
+// left to bf16.  smem: 8 ints.
+constexpr int kNoShift = 1 << 20;
 template <int BM, int THREADS>
-__device__ inline bool f16_holds(const Args& p, const Place& at) {
-  int bad = 0;
+__device__ inline int f16_shift(const Args& p, const Place& at, int* smem) {
+  int high = 0, low = 0;  // the largest byte, and 255 - the least that is not 0
   const long long g0 = at.rb / 64, n = (at.re + 63) / 64 - g0;
   for (int step = at.m0 / 128; 128 * step < min(at.m0 + BM, p.x_row); ++step) {
     const unsigned* sc = reinterpret_cast<const unsigned*>(p.x_scales) + ((long long)step * p.x_groups + g0) * 64;
@@ -625,12 +642,29 @@ __device__ inline bool f16_holds(const Args& p, const Place& at) {
       const unsigned w = sc[i];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const unsigned b = (w >> (8 * e)) & 0xffu;
-        bad |= b != 0 && (b < 112 || b > 134);
+        const int b = (int)((w >> (8 * e)) & 0xffu);
+        high = max(high, b);
+        low = max(low, b != 0 ? 255 - b : 0);
       }
     }
   }
-  return !__syncthreads_or(bad);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    high = max(high, __shfl_xor(high, d));
+    low = max(low, __shfl_xor(low, d));
+  }
+  if ((threadIdx.x & 63) == 0) smem[threadIdx.x >> 6] = high << 8 | low;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    high = max(high, smem[w] >> 8);
+    low = max(low, smem[w] & 0xff);
+  }
+  __syncthreads();  // the stages overwrite smem
+  high = __builtin_amdgcn_readfirstlane(high);
+  low = 255 - __builtin_amdgcn_readfirstlane(low);
+  if (high == 255 || high - low > 22) return kNoShift;
+  return high == 0 || (low >= 112 && high <= 134) ? 0 : 134 - high;
 }
 
 constexpr int larger(int a, int b) { return a > b ? a : b; }
@@ -640,9 +674,11 @@ template <int KIND, int TILE>
 __global__ __launch_bounds__(2 * TILE, 2) void mx_dw_staged_kernel(Args p) {
   constexpr int OTHER = KIND == kF16 ? kF16Planes : KIND, WGN = TILE / 64;
   __shared__ __attribute__((aligned(16))) unsigned short smem[larger(staged_lds<KIND, TILE, TILE>(), staged_lds<OTHER, TILE, TILE>())];
-  const Place at = place<TILE, TILE>(p);
+  Place at = place<TILE, TILE>(p);
   if constexpr (KIND == kF16) {
-    if (!f16_holds<TILE, 2 * TILE>(p, at)) return staged_body<kF16Planes, TILE, TILE, 2, WGN>(p, at, smem);
+    const int shift = f16_shift<TILE, 2 * TILE>(p, at, reinterpret_cast<int*>(smem));
+    if (shift == kNoShift) return staged_body<kF16Planes, TILE, TILE, 2, WGN>(p, at, smem);
+    at.shift = shift;
   }
   staged_body<KIND, TILE, TILE, 2, WGN>(p, at, smem);
 }
@@ -650,9 +686,11 @@ __global__ __launch_bounds__(2 * TILE, 2) void mx_dw_staged_kernel(Args p) {
 template <bool F16>
 __global__ __launch_bounds__(512) void mx_dw_direct_kernel(Args p) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[larger(2 * 64 * 512, staged_lds<kF16Planes, 256, 256>())];
-  const Place at = place<256, 256>(p);
+  Place at = place<256, 256>(p);
   if constexpr (F16) {
-    if (!f16_holds<256, 512>(p, at)) return staged_body<kF16Planes, 256, 256, 2, 4>(p, at, smem);
+    const int shift = f16_shift<256, 512>(p, at, reinterpret_cast<int*>(smem));
+    if (shift == kNoShift) return staged_body<kF16Planes, 256, 256, 2, 4>(p, at, smem);
+    at.shift = shift;
   }
   direct_body<F16, 256, 256, 2, 4>(p, at, smem);
 }

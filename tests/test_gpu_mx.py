@@ -389,6 +389,20 @@ def test_dw_f16_scales_beyond_f16_in_large_tiles(gpu):
     check_dw(gpu, 300, 4100, 4096, "f16", x=x)
 
 
+@pytest.mark.parametrize("rows,K,N", [(1, 5, 3), (100, 300, 50), (700, 300, 129), (5000, 100, 64), (300, 4100, 4096)])
+@pytest.mark.parametrize("power,span", [(-100, 0), (-100, 22), (-100, 23), (-30, 21), (60, 0), (60, 22), (60, 23)])
+def test_dw_f16_scales_of_any_size(gpu, rows, K, N, power, span):
+    """Scales all small or all large, over the 22 powers of two that f16 holds at once and over one more; blocks of zeros."""
+    rng = np.random.default_rng(1000 + rows + power + span)
+    x = rng.normal(size=(rows, K)).astype(np.float32)
+    x[rng.random((rows, K)) < 0.3] = 0
+    x = np.clip(np.ldexp(x, power), -np.ldexp(1.0, power), np.ldexp(1.0, power)).astype(np.float32)
+    x[rng.integers(0, rows, 4)] *= np.float32(2.0 ** span)  # whole rows
+    x[rng.integers(0, rows, max(1, rows // 5))] = 0
+    x[rows // 2] = np.float32(2.0 ** (power + span))
+    check_dw(gpu, rows, K, N, "f16", x=x)
+
+
 @pytest.mark.parametrize("rows,K,N", [(100, 60, 50), (300, 2000, 2048)])
 def test_dw_subnormal_values(gpu, rows, K, N):
     """Halves down to their last bit; f32 down to 2^-133, the last bit of a bf16; 8-bit values far below f16's range."""
