@@ -570,3 +570,31 @@ def test_a_quantized_layer_in_a_row(gpu):
         xv = X.quantize(x, G.MXFP8)[2]
         tol = 308 * 2.0 ** -23 * (np.abs(xv) @ np.abs(wv).T + np.abs(bias))
         assert np.all(np.abs(gpu.download(y) - np.maximum(xv @ wv.T + bias, 0)) <= tol)
+
+
+def test_two_contexts_at_once_and_again(gpu):
+    """Workspaces are a context's own and sums have a fixed order: results of two contexts whose calls are in flight
+    together, over and over, are those of one call, bit for bit."""
+    rng = np.random.default_rng(21)
+    x, w = X.values(rng, 3000, 300), rng.normal(size=(200, 300)).astype(np.float32)
+    d = rng.normal(size=(3000, 200)).astype(np.float32)
+    other = G.Gpu(0)
+    runs = []
+    for g in (gpu, other):
+        q, w4 = g.zeros((3000, 300), G.MXFP8), g.zeros((200, 300), G.MXFP4)
+        g.convert(g.upload(x), q)
+        g.convert(g.upload(w), w4)
+        runs.append((g, q, w4, {t: g.upload(d, DTYPE[t]) for t in DTYPE}))
+        g.sync()
+    got = []
+    for _ in range(4):
+        for g, q, w4, ds in runs:
+            y = g.empty((3000, 200))
+            g.gemm(G.NT, q, w4, y)
+            grads = [g.empty((300, 200)) for _ in DTYPE] + [g.empty((1, 200)) for _ in DTYPE]
+            for i, t in enumerate(sorted(DTYPE)):
+                g.matmul_at_b(q, ds[t], grads[i], colsum=grads[3 + i])
+            got.append((g, [y] + grads))
+    values = [[g.download(t) for t in ts] for g, ts in got]
+    for v in values[1:]:
+        assert all(np.array_equal(a, b) for a, b in zip(v, values[0]))
