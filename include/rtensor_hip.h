@@ -110,8 +110,8 @@ int rt_buf_info(const rt_buf* buf, rt_dtype* dtype, size_t* shape, int* rank);
 int rt_upload_labels(rt_ctx* ctx, const uint64_t* labels, size_t n, rt_buf** out);
 /* A buffer over device memory that the caller owns: a tensor of another library,
  * a slice of the caller's arena.  ptr is on the context's device, aligned to the
- * element (RT_MXFP*: to 16 bytes), with rt_tensor_bytes bytes inside one
- * allocation.  rt_free gives up the handle only.  The memory outlives the handle
+ * element (RT_MXFP* and the batch of a training plan: to 16 bytes), with
+ * rt_tensor_bytes bytes inside one allocation.  rt_free gives up the handle only.  The memory outlives the handle
  * and the work enqueued on it, and the caller orders other streams' use of it
  * against the context's (rt_sync, or a device synchronisation). */
 int rt_wrap(rt_ctx* ctx, rt_dtype dtype, const size_t* shape, int rank, void* ptr, rt_buf** out);

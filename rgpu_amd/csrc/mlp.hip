@@ -687,6 +687,9 @@ static int check_inputs(rt_mlp* p, const rt_buf* x) {
   if (x == nullptr) return fail(c, RT_ERR_INVALID, "null batch");
   const rt_dtype want = p->mixed ? RT_BF16 : RT_F32;
   if (x->dtype != want) return fail(c, RT_ERR_DTYPE, "batch must be %s", p->mixed ? "bf16" : "f32");
+  // The plan's launches were laid out for such a batch; only rt_wrap makes others.
+  if (reinterpret_cast<uintptr_t>(x->ptr) % 16 != 0)
+    return fail(c, RT_ERR_INVALID, "batch must be aligned to 16 bytes");
   if (x->n != p->batch * p->L[0].din)
     return fail(c, RT_ERR_SHAPE, "batch with %zu elements, plan built for %zu", x->n, p->batch * p->L[0].din);
   return RT_OK;

@@ -145,6 +145,23 @@ def test_wrap(gpu):
     assert np.array_equal(t.cpu().numpy(), 4 * np.arange(64, dtype=np.float32))
 
 
+def test_wrapped_batch_of_a_plan(gpu):
+    """A batch in the caller's memory trains as an uploaded one does; one that the plan's kernels cannot take is refused
+    before anything runs."""
+    rng = np.random.default_rng(2)
+    params = [rng.normal(size=s).astype(np.float32) / 8 for s in ((64, 96), (1, 96), (96, 10), (1, 10))]
+    t = torch.tensor(rng.normal(size=(4 + 40 * 64,)), dtype=torch.float32, device="cuda")
+    torch.cuda.synchronize()
+    labels = G.upload_labels(gpu, rng.integers(0, 10, 40))
+    plain, wrapped = (G.GpuMlp.from_params(gpu, params, 40, 1e-3) for _ in range(2))
+    plain.step(gpu.upload(t.cpu().numpy()[4 : 4 + 40 * 64].reshape(40, 64)), labels)
+    odd = gpu.wrap(t.data_ptr() + 4, (40, 64), owner=t)
+    assert status(wrapped.step, odd, labels) == "RT_ERR_INVALID"
+    assert status(wrapped.forward_only, odd) == "RT_ERR_INVALID"
+    wrapped.step(gpu.wrap(t.data_ptr() + 16, (40, 64), owner=t), labels)
+    assert all(np.array_equal(a, b) for a, b in zip(plain.weights(), wrapped.weights()))
+
+
 # ------------------------------------------------------------------ conversion
 SHAPES = [(1, 1), (1, 32), (1, 5000), (3, 33), (2, 31), (64, 128), (65, 129), (100, 1003), (130, 64), (300, 520)]
 
