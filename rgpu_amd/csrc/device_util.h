@@ -69,14 +69,19 @@ __device__ inline void dma16(__amdgpu_buffer_rsrc_t rsrc, void* lds, int voff, i
 // bookkeeping: the caller's own wait_vm before its barrier is then the only
 // ordering, and a caller must wait_vm<0>() before reusing the LDS it targets.
 // M0 (the LDS destination) is set inside the asm; kernels that use this form
-// must not also use the builtin, which may keep M0 live across it.
+// must not also use the builtin, which may keep M0 live across it.  A load that
+// takes its destination from M0 wants one wait state after a scalar write of it
+// (the compiler puts an s_nop 0 there for the builtin, and does not look into
+// asm).  Here it stands as its encoding, .long 0xbf800000, because the check of
+// these kernels' assembly reads instructions by name and wants M0's write next
+// to the load.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ inline void dma16_asm(__amdgpu_buffer_rsrc_t rsrc, void* lds, int voff, int soff) {
   const int so = __builtin_amdgcn_readfirstlane(soff);
   const unsigned dst = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) void*)lds);
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(dst), "v"(voff), "s"(rsrc),
-               "s"(so)
+  asm volatile("s_mov_b32 m0, %0\n\t.long 0xbf800000\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(dst), "v"(voff),
+               "s"(rsrc), "s"(so)
                : "m0");
 }
 
@@ -88,11 +93,13 @@ __device__ inline unsigned lds_offset(void* lds) {
 }
 __device__ inline void dma16_at(__amdgpu_buffer_rsrc_t rsrc, unsigned dst, int voff) {
   const unsigned d = __builtin_amdgcn_readfirstlane(dst);
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(d), "v"(voff), "s"(rsrc) : "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(d), "v"(voff), "s"(rsrc)
+               : "m0");
 }
 __device__ inline void dma4_at(__amdgpu_buffer_rsrc_t rsrc, unsigned dst, int voff) {
   const unsigned d = __builtin_amdgcn_readfirstlane(dst);
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(d), "v"(voff), "s"(rsrc) : "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(d), "v"(voff), "s"(rsrc)
+               : "m0");
 }
 #pragma clang diagnostic pop
 
