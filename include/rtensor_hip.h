@@ -153,10 +153,9 @@ int rt_convert_t(rt_ctx* ctx, const rt_buf* src, rt_buf* dst);
  * With microscaled operands (no counterpart in the reference):
  *   - RT_NT, B RT_MXFP4 [N, K], A RT_MXFP4 or RT_MXFP8 [M, K], C f32 or bf16, no
  *     epilogue, RT_EPI_BIAS or RT_EPI_BIAS_RELU, K <= 2^22: the values of the
- *     codes are multiplied and added in f32.  With an 8-bit A and a bf16 C a
- *     product may lose up to 2^-13 of the largest of the eight that share its
- *     columns 8 j .. 8 j + 7, of whose factors the 8-bit one was rounded by up to
- *     2^-5 when it was converted.
+ *     codes are multiplied and added in f32; a bf16 C is that sum rounded once.
+ *     The order of the additions goes by the sizes: a row of C may differ in the
+ *     last bits of its sums between a product of few rows and one of many.
  *   - RT_TN, A RT_MXFP8 [K, M], B f32, bf16 or f16 [K, N], C f32, no epilogue,
  *     with or without colsum, M and N <= 2^22: the weight gradient from an input
  *     that was saved in 8 bits.  Products are exact (of an f32 B its bits below

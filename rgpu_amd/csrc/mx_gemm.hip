@@ -7,14 +7,12 @@
 // window that reaches 2^-13 below the power of two of the largest (measured: of
 // 2^16 - 2^16 + 2^s in one eight nothing below s = 3 comes back; between eights
 // and against the accumulator 2^-24).  4-bit products span 2^-2 to 36 and fit.
-// An 8-bit A does not (its values span 2^-9 to 448).  For an f32 C each of its
-// fragments therefore goes in as two, the codes from 2 up and those below, with
-// zeros in the others' places: products then reach from 2^-3 to below 2^12, or
-// from 2^-10 to below 2^4, the sums of eight are exact, and what is left are
-// f32 additions.  For a bf16 C it goes in whole (SPLIT false): what is dropped
-// is at most 2^-13 of a neighbouring product, whose 8-bit factor was itself
-// rounded by up to 2^-5 of it, and half the work is saved (8192 x 4096, K 4096:
-// 193 us split, 116 whole).
+// An 8-bit A does not (its values span 2^-9 to 448).  Each of its fragments
+// therefore goes in as two, the codes from 2 up and those below, with zeros in the
+// others' places: products then reach from 2^-3 to below 2^12, or from 2^-10 to
+// below 2^4, the sums of eight are exact, and what is left are f32 additions.
+// Also for a bf16 C, which is the f32 one rounded once: A in one piece (8192 x
+// 4096, K 4096: 116 us, 193 in two) changed one value in 500 of 4100 x 1000, K 4000.
 //
 // What a lane holds.  Lane (g, r), g = lane / 16, r = lane % 16, of an operand
 // of 16 rows takes row r: the 4-bit codes of columns 32 g .. 32 g + 31 (16
@@ -38,8 +36,8 @@
 // steps by the layout.
 //
 // Measured: 4 bits, 8192 x 16384, K 4096, bf16 C, 298 us (3.7 PFLOP/s; its 268 MB
-// of C at the copy rate take 52); 8 bits, 8192 x 4096, K 4096, 120 us (2.3
-// PFLOP/s); one row by 4096 x 4096 weights 4.4 us, of which a launch is 3.2.
+// of C at the copy rate take 52); 8 bits, 8192 x 4096, K 4096, 193-241 us (1.1 to
+// 1.4 PFLOP/s); one row by 4096 x 4096 weights 4.4 us, of which a launch is 3.2.
 
 #include <algorithm>
 #include <type_traits>
@@ -106,7 +104,7 @@ struct Frag {
 
 // acc[u] += (B_u·Aᵀ of one step) for TN operands B; SA: which byte of A's scale
 // dword (B's: u % 4).
-template <int ABITS, bool SPLIT, int SA, int TN>
+template <int ABITS, int SA, int TN>
 __device__ inline void mfma_row(const Frag<ABITS>& a, const Frag<4> (&b)[TN], f4 (&acc)[TN], unsigned sa,
                                 const unsigned (&sb)[(TN + 3) / 4]) {
   auto one = [&](const Frag<ABITS>& x) {
@@ -116,8 +114,7 @@ __device__ inline void mfma_row(const Frag<ABITS>& a, const Frag<4> (&b)[TN], f4
                                                                 (int)sb[u / 4], SA, (int)sa);
     });
   };
-  if constexpr (SPLIT) {
-    static_assert(ABITS == 8, "4-bit products need no split");
+  if constexpr (ABITS == 8) {
     one(a.part(false));
     one(a.part(true));
   } else {
@@ -259,7 +256,7 @@ __device__ __forceinline__ void store_rows(const Args& p, const f4 (&acc)[TM][TN
 }
 
 // Block tile BM x BN, WGM x WGN waves, NS stages.
-template <int ABITS, bool SPLIT, int BM, int BN, int WGM, int WGN, int NS>
+template <int ABITS, int BM, int BN, int WGM, int WGN, int NS>
 __global__ __launch_bounds__(64 * WGM * WGN) void mx_gemm_kernel(Args p) {
   constexpr int WAVES = WGM * WGN, WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   using A = Side<ABITS, BM, WAVES>;
@@ -338,7 +335,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mx_gemm_kernel(Args p) {
   auto mfmas = [&](const Set& s) {
     static_for<0, TM>([&](auto tc) {
       constexpr int t = decltype(tc)::value;
-      mfma_row<ABITS, SPLIT, t & 3, TN>(s.a[t], s.b, acc[t], s.as[t / 4], s.bs);
+      mfma_row<ABITS, t & 3, TN>(s.a[t], s.b, acc[t], s.as[t / 4], s.bs);
     });
   };
 
@@ -439,7 +436,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void mx_rows_kernel(Args p) {
       if (k0 + i < p.steps) {
         static_for<0, TM>([&](auto tc) {
           constexpr int t = decltype(tc)::value;
-          mfma_row<ABITS, ABITS == 8, t & 3, 1>(fa[i][t], fb[i], acc[t], sa[i], sb[i]);
+          mfma_row<ABITS, t & 3, 1>(fa[i][t], fb[i], acc[t], sa[i], sb[i]);
         });
       }
     }
@@ -456,11 +453,11 @@ __global__ __launch_bounds__(64 * kRowWaves) void mx_rows_kernel(Args p) {
   }
 }
 
-template <int ABITS, bool SPLIT, int BM, int BN, int WGM, int WGN, int NS>
+template <int ABITS, int BM, int BN, int WGM, int WGN, int NS>
 hipError_t launch_tiles(hipStream_t s, Args p) {
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
-  rt::launch(mx_gemm_kernel<ABITS, SPLIT, BM, BN, WGM, WGN, NS>,
+  rt::launch(mx_gemm_kernel<ABITS, BM, BN, WGM, WGN, NS>,
              dim3((unsigned)((long long)p.tiles_m * p.tiles_n)), dim3(64 * WGM * WGN), 0, s, p);
   return hipGetLastError();
 }
@@ -469,29 +466,30 @@ hipError_t launch_tiles(hipStream_t s, Args p) {
 // takes whole rounds of 256, or a last one that leaves no more than a third of
 // all places idle (us with 256 and 128 tiles: 4096 x 4096, K 1024, 256 blocks,
 // 19.0 and 21.1; K 4096: 6912 x 4864, 513 blocks, 104 and 110; 4608 x 4096, 288
-// blocks, 66 and 56).  128 x 128, two a CU, from 208 blocks on (1800 x 1800, K 2000, 225 blocks,
-// 8 bits: 13.2 and 13.9 with 64 tiles; 700 x 4096, K 1000, 192 blocks: 12.0 and
-// 10.6).  For 8 bits larger tiles were no faster (256 x 128, 8192 x 4096, K 4096:
-// 119.7 and 115.9 with 128).
-template <int ABITS, bool SPLIT>
+// blocks, 66 and 56).  128 x 128, two a CU, from 208 blocks on (8 bits, us with 128
+// and 64 tiles: 1800 x 1800, K 2000, 225 blocks, 20.8 and 24.7; 2048 x 4096, K
+// 1024, 512 blocks, 23.2 and 30.6; 700 x 4096, K 1000, 192 blocks, 13.1 and 12.0).
+template <int ABITS>
 hipError_t launch_many(hipStream_t s, const Args& p) {
   auto tiles = [&](int t) { return (long long)((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
   if constexpr (ABITS == 4) {
     const long long t = tiles(256), places = (t + 255) / 256 * 256;
-    if (t >= 256 && 2 * places <= 3 * t) return launch_tiles<4, false, 256, 256, 2, 4, 4>(s, p);
+    if (t >= 256 && 2 * places <= 3 * t) return launch_tiles<4, 256, 256, 2, 4, 4>(s, p);
   }
-  if (tiles(128) >= 208) return launch_tiles<ABITS, SPLIT, 128, 128, 2, 2, 3>(s, p);
-  return launch_tiles<ABITS, SPLIT, 64, 64, 2, 2, 4>(s, p);
+  if (tiles(128) >= 208) return launch_tiles<ABITS, 128, 128, 2, 2, 3>(s, p);
+  return launch_tiles<ABITS, 64, 64, 2, 2, 4>(s, p);
 }
 
 // Few rows stay with the kernel that reads B once and A again for every 16
-// columns, up to 48, or 64 over a short K (N 4096, 8 bits, us there and with 64
-// tiles: 16 rows, K 4096, 5.0 and 8.0; 33 rows 7.7 and 8.1; 64 rows 11.2 and 8.1,
-// K 1024 5.4 and 5.7).
+// columns, up to 48, or 64 over a short K, or for 8 bits where its blocks are one
+// round of the CUs (8 bits, us there and with 64 tiles: N 4096, K 4096, 49 rows 11.1
+// and 15.0, 64 rows 12.6 and 15.0; N 1000, K 4000, 64 rows 11.9 and 14.7; N 16384,
+// K 4096, 64 rows 43.4 and 16.8.  4 bits, N 4096, 64 rows: K 1024 4.7 with 64 tiles).
 template <int ABITS>
 hipError_t launch(hipStream_t s, const Args& p) {
   // (A grid holds fewer than 2^32 threads.)
-  if ((p.M <= 48 || (p.M <= 64 && p.steps <= 8)) && p.N <= (1 << 26)) {
+  const bool one_round = ABITS == 8 && p.N <= 16 * 256;
+  if ((p.M <= 48 || (p.M <= 64 && (p.steps <= 8 || one_round))) && p.N <= (1 << 26)) {
     const dim3 grid((unsigned)((p.N + 15) / 16)), block(64 * kRowWaves);
     const int tm = (p.M + 15) / 16;
     if (tm == 1) rt::launch(mx_rows_kernel<ABITS, 1>, grid, block, 0, s, p);
@@ -500,10 +498,7 @@ hipError_t launch(hipStream_t s, const Args& p) {
     else rt::launch(mx_rows_kernel<ABITS, 4>, grid, block, 0, s, p);
     return hipGetLastError();
   }
-  if constexpr (ABITS == 8) {
-    if (!p.out_bf16) return launch_many<8, true>(s, p);
-  }
-  return launch_many<ABITS, false>(s, p);
+  return launch_many<ABITS>(s, p);
 }
 
 }  // namespace
