@@ -243,6 +243,8 @@ class GpuTensor:
 
     def free(self):
         if self.handle and self.gpu._h and not self.gpu._keep(self):
+            if self.owner is not None:
+                self.gpu._hold(self.owner, self.nbytes)
             self.gpu._call("rt_free", self.gpu._h, self.handle)
         self.handle = None
         self.owner = None
@@ -274,7 +276,11 @@ class Gpu:
         # reason as the library's own cache: the context's work runs in order
         # on its one stream.
         self._spare = {}
+        # Owners of wrapped memory whose tensors are gone, kept until the work
+        # that was enqueued on them is done.
+        self._held, self._held_bytes, self._mark = [], 0, None
 
+    _HELD_MAX, _HELD_MAX_BYTES = 256, 1 << 30
     _SPARE_PER_SHAPE = 8
     _SPARE_MAX_BYTES = 64 << 20
 
@@ -287,11 +293,34 @@ class Gpu:
         lst.append(t.handle)
         return True
 
+    def _hold(self, owner, nbytes: int) -> None:
+        """Keep what owns wrapped memory until the stream has been waited for
+        (every call that does lets go of it); past a bound, wait here."""
+        self._held.append(owner)
+        self._held_bytes += nbytes
+        if len(self._held) >= self._HELD_MAX or self._held_bytes >= self._HELD_MAX_BYTES:
+            if self._mark is None:
+                t = self.zeros((1,))
+                self._mark, t.handle = t.handle, None  # the handle alone: a tensor would refer back here
+            # Unlike rt_sync a download leaves the label flag to the program.
+            self._drain("rt_download", self._h, self._mark, C.byref(C.c_float()), 4)
+
+    def _drain(self, name: str, *args) -> None:
+        """A call that returns once the stream's work is done."""
+        held, bytes_, self._held, self._held_bytes = self._held, self._held_bytes, [], 0
+        try:
+            self._call(name, *args)
+        except RtError as e:
+            if e.status != "RT_ERR_LABEL":  # that one is reported after the wait
+                self._held, self._held_bytes = held + self._held, bytes_ + self._held_bytes
+            raise
+
     def close(self):
         if self._h:
             self._spare = {}  # the context frees every buffer it still owns
             lib().rt_close(self._h)
-            self._h = None
+            self._h = self._mark = None
+            self._held, self._held_bytes = [], 0
 
     def __del__(self):
         try:
@@ -312,7 +341,7 @@ class Gpu:
         return buf.value.decode()
 
     def sync(self) -> None:
-        self._call("rt_sync", self._h)
+        self._drain("rt_sync", self._h)
 
     # --------------------------------------------------------------- buffers
     def zeros(self, shape, dtype: int = F32) -> GpuTensor:
@@ -336,9 +365,9 @@ class Gpu:
     def wrap(self, ptr: int, shape, dtype: int = F32, owner=None) -> GpuTensor:
         """A tensor over device memory that something else owns (rt_wrap),
         such as ``t.data_ptr()`` of a contiguous torch tensor t on this device.
-        ``owner`` is kept as long as the handle.  Order the context's stream
-        against others that use the memory (``sync``, a device
-        synchronisation)."""
+        ``owner`` is kept as long as the handle, and until the work that was
+        enqueued on it is done.  Order the context's stream against others
+        that use the memory (``sync``, a device synchronisation)."""
         shape = _shape(shape)
         arr = (C.c_size_t * max(len(shape), 1))(*shape)
         h = C.c_void_p()
@@ -375,7 +404,8 @@ class Gpu:
 
     def download(self, t: GpuTensor) -> np.ndarray:
         out = np.empty(t.nbytes, np.uint8) if t.dtype in (MXFP4, MXFP8) else np.empty(t.shape, _np_dtype(t.dtype))
-        self._call("rt_download", self._h, t.handle, out.ctypes.data_as(C.c_void_p), out.nbytes)
+        (self._drain if out.nbytes else self._call)("rt_download", self._h, t.handle, out.ctypes.data_as(C.c_void_p),
+                                                    out.nbytes)
         return out
 
     def download_f32(self, t: GpuTensor) -> np.ndarray:
