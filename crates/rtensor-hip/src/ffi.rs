@@ -113,6 +113,8 @@ extern "C" {
     pub fn rt_upload_labels(ctx: *mut RtCtx, labels: *const u64, n: usize, out: *mut *mut RtBuf) -> c_int;
     pub fn rt_wrap(ctx: *mut RtCtx, dtype: c_int, shape: *const usize, rank: c_int, ptr: *mut c_void,
                    out: *mut *mut RtBuf) -> c_int;
+    pub fn rt_order_after(ctx: *mut RtCtx, stream: *mut c_void) -> c_int;
+    pub fn rt_order_before(ctx: *mut RtCtx, stream: *mut c_void) -> c_int;
     pub fn rt_tensor_bytes(dtype: c_int, shape: *const usize, rank: c_int) -> usize;
     pub fn rt_convert(ctx: *mut RtCtx, src: *const RtBuf, dst: *mut RtBuf) -> c_int;
     pub fn rt_convert_t(ctx: *mut RtCtx, src: *const RtBuf, dst: *mut RtBuf) -> c_int;

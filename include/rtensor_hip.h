@@ -111,10 +111,19 @@ int rt_upload_labels(rt_ctx* ctx, const uint64_t* labels, size_t n, rt_buf** out
 /* A buffer over device memory that the caller owns: a tensor of another library,
  * a slice of the caller's arena.  ptr is on the context's device, aligned to the
  * element (RT_MXFP* and the batch of a training plan: to 16 bytes), with
- * rt_tensor_bytes bytes inside one allocation.  rt_free gives up the handle only.  The memory outlives the handle
- * and the work enqueued on it, and the caller orders other streams' use of it
- * against the context's (rt_sync, or a device synchronisation). */
+ * rt_tensor_bytes bytes inside one allocation.  rt_free gives up the handle only.
+ * The memory outlives the handle and the work enqueued on it, and the caller
+ * orders other streams' use of it against the context's, which no stream is
+ * ordered with by itself (rt_order_after, rt_order_before, rt_sync, or a device
+ * synchronisation). */
 int rt_wrap(rt_ctx* ctx, rt_dtype dtype, const size_t* shape, int rank, void* ptr, rt_buf** out);
+/* Orders the context's work with a stream of the caller's (a hipStream_t of the
+ * context's device, NULL for the default one) without waiting on the host:
+ * rt_order_after has what the context enqueues from now on wait for what the
+ * stream holds now, rt_order_before has what the stream is given from now on wait
+ * for what the context has enqueued.  A stream that is being captured is refused. */
+int rt_order_after(rt_ctx* ctx, void* stream);
+int rt_order_before(rt_ctx* ctx, void* stream);
 /* Bytes of a tensor (what rt_upload and rt_download move); 0 for a bad dtype or
  * shape, and for a tensor without elements. */
 size_t rt_tensor_bytes(rt_dtype dtype, const size_t* shape, int rank);

@@ -58,6 +58,8 @@ struct rt_ctx {
   // Host-to-device copies of staged batches (rt_mlp_load), created on first
   // use; default priority like the main stream.
   hipStream_t copy_stream = nullptr;
+  // What rt_order_after and rt_order_before record, created on first use.
+  hipEvent_t order = nullptr;
   // This device's copy of rt_gemm_splitk_static's static scratch array.
   float* static_scratch = nullptr;
 };

@@ -188,6 +188,7 @@ int rt_close(rt_ctx* c) {
   for (auto e : c->event_pool) hipEventDestroy(e);
   if (c->timer0) hipEventDestroy(c->timer0);
   if (c->timer1) hipEventDestroy(c->timer1);
+  if (c->order) hipEventDestroy(c->order);
   hipFree(c->d_flags);
   if (c->scratch) hipFree(c->scratch);
   if (c->copy_stream) hipStreamDestroy(c->copy_stream);
@@ -370,6 +371,34 @@ int rt_wrap(rt_ctx* c, rt_dtype dtype, const size_t* shape, int rank, void* ptr,
   c->bufs.insert(b);
   *out = b;
   return RT_OK;
+}
+
+// `later` waits for what `earlier` holds now; one of the two is the caller's stream.
+static int order_streams(rt_ctx* c, hipStream_t theirs, hipStream_t earlier, hipStream_t later) {
+  hipDevice_t device = c->device;
+  if (theirs != nullptr) HIP_TRY(c, hipStreamGetDevice(theirs, &device), "stream device");
+  if (device != c->device)
+    return fail(c, RT_ERR_INVALID, "a stream of device %d, the context's is %d", (int)device, c->device);
+  // An event of a captured stream would put the context's stream into the capture.
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(theirs, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
+    (void)hipGetLastError();
+    return fail(c, RT_ERR_INVALID, "a stream that is being captured cannot be ordered with a context");
+  }
+  if (!c->order) HIP_TRY(c, hipEventCreateWithFlags(&c->order, hipEventDisableTiming), "event");
+  HIP_TRY(c, hipEventRecord(c->order, earlier), "event record");
+  HIP_TRY(c, hipStreamWaitEvent(later, c->order, 0), "stream wait");
+  return RT_OK;
+}
+
+int rt_order_after(rt_ctx* c, void* stream) {
+  CHECK_CTX(c);
+  return order_streams(c, static_cast<hipStream_t>(stream), static_cast<hipStream_t>(stream), c->stream);
+}
+
+int rt_order_before(rt_ctx* c, void* stream) {
+  CHECK_CTX(c);
+  return order_streams(c, static_cast<hipStream_t>(stream), c->stream, static_cast<hipStream_t>(stream));
 }
 
 int rt_zeros(rt_ctx* c, rt_dtype dtype, const size_t* shape, int rank, rt_buf** out) {

@@ -71,6 +71,8 @@ SIGNATURES = {
     "rt_buf_info": (C.c_int, [_VP, C.POINTER(C.c_int), _SZP, C.POINTER(C.c_int)]),
     "rt_upload_labels": (C.c_int, [_VP, C.POINTER(C.c_uint64), C.c_size_t, C.POINTER(_VP)]),
     "rt_wrap": (C.c_int, [_VP, C.c_int, _SZP, C.c_int, _VP, C.POINTER(_VP)]),
+    "rt_order_after": (C.c_int, [_VP, _VP]),
+    "rt_order_before": (C.c_int, [_VP, _VP]),
     "rt_tensor_bytes": (C.c_size_t, [C.c_int, _SZP, C.c_int]),
     "rt_convert": (C.c_int, [_VP, _VP, _VP]),
     "rt_convert_t": (C.c_int, [_VP, _VP, _VP]),
@@ -367,12 +369,26 @@ class Gpu:
         such as ``t.data_ptr()`` of a contiguous torch tensor t on this device.
         ``owner`` is kept as long as the handle, and until the work that was
         enqueued on it is done.  Order the context's stream against others
-        that use the memory (``sync``, a device synchronisation)."""
+        that use the memory (``order_after`` and ``order_before``; or
+        ``sync``, a device synchronisation)."""
         shape = _shape(shape)
         arr = (C.c_size_t * max(len(shape), 1))(*shape)
         h = C.c_void_p()
         self._call("rt_wrap", self._h, dtype, arr, len(shape), C.c_void_p(ptr), C.byref(h))
         return GpuTensor(self, h.value, shape, dtype, owner, True)
+
+    def order_after(self, stream: int = 0) -> None:
+        """What is enqueued here from now on waits for what ``stream`` holds
+        now, a HIP stream of this device such as
+        ``torch.cuda.current_stream().cuda_stream`` (0: the default one):
+        before calls that read or write memory which that stream's work
+        writes or reads."""
+        self._call("rt_order_after", self._h, C.c_void_p(stream))
+
+    def order_before(self, stream: int = 0) -> None:
+        """What ``stream`` is given from now on waits for what has been
+        enqueued here: after the last call on memory that it uses next."""
+        self._call("rt_order_before", self._h, C.c_void_p(stream))
 
     def upload(self, a, dtype: Optional[int] = None, shape=None) -> GpuTensor:
         """Upload a host array.  dtype BF16 takes f32 values (rounded to

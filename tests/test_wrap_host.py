@@ -93,3 +93,7 @@ def test_tensors_of_the_library_hold_nothing():
     gpu.zeros((4,)).free()
     gpu.wrap(256, (4,)).free()
     assert not gpu._held and isinstance(gpu.download(gpu.zeros((2,))), np.ndarray)
+
+
+def test_null_handles():
+    assert G.lib().rt_order_after(None, None) == 2 and G.lib().rt_order_before(None, None) == 2
