@@ -283,6 +283,9 @@ def _call(s):
     case, gpu = s["case"], _gpu()
     if "handles" not in s:
         s["handles"] = _handles(s)
+        # The inputs were made on torch's stream, which the context's is not ordered with; what the calls below write is
+        # read by others once the device has been waited for.
+        gpu.order_after(torch.cuda.current_stream().cuda_stream)
     h = s["handles"]
     if case["kind"] == "quantize":
         if case["transposed"]:
