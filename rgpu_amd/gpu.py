@@ -187,7 +187,7 @@ def mx_decode(data, shape, dtype: int) -> np.ndarray:
     at = -(-rows * row_bytes // 256) * 256
     code = data[:rows * row_bytes].reshape(rows, row_bytes)
     if dtype == MXFP4:
-        code = np.stack([code & 15, code >> 4], axis=2).reshape(rows, -1)
+        code = np.stack([code & 15, code >> 4], axis=2).reshape(rows, 2 * row_bytes)
         value = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6], np.float32)[code & 7]
         negative = code >= 8
     else:
@@ -201,8 +201,8 @@ def mx_decode(data, shape, dtype: int) -> np.ndarray:
     scale = scale.reshape(groups * 64, steps * 4)[:rows].astype(np.int32)
     factor = np.where(scale == 255, np.float32(np.nan), np.ldexp(np.float32(1), np.minimum(scale, 254) - 127))
     with np.errstate(over="ignore"):  # an MXFP4 element from 2^128 on
-        out = value.reshape(rows, -1, 32) * factor.astype(np.float32)[:, :, None]
-    return out.reshape(rows, -1)[:, :cols]
+        out = value.reshape(rows, 4 * steps, 32) * factor.astype(np.float32)[:, :, None]
+    return out.reshape(rows, 128 * steps)[:, :cols]
 
 
 def _shape(shape) -> tuple:

@@ -40,3 +40,10 @@ def test_null_handles():
     L = G.lib()
     assert L.rt_convert_t(None, None, None) == 2
     assert L.rt_wrap(None, G.F32, None, 0, None, None) == 2
+
+
+@pytest.mark.parametrize("fmt", [G.MXFP4, G.MXFP8])
+@pytest.mark.parametrize("shape", [(0, 5), (5, 0), (0, 0)])
+def test_decoder_of_no_elements(shape, fmt):
+    got = G.mx_decode(np.zeros(0, np.uint8), shape, fmt)
+    assert got.shape == shape and got.dtype == np.float32
