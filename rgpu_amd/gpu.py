@@ -450,7 +450,7 @@ class Gpu:
     def gemm(self, layout: int, a: GpuTensor, b: GpuTensor, c: GpuTensor, epi: int = EPI_NONE,
              aux: Optional[GpuTensor] = None, colsum: Optional[GpuTensor] = None) -> None:
         self._call("rt_gemm", self._h, layout, a.handle, b.handle, c.handle, epi,
-                   aux.handle if aux else None, colsum.handle if colsum else None)
+                   aux.handle if aux is not None else None, colsum.handle if colsum is not None else None)
 
     def matmul(self, a, b, c):
         """C = A·B (op_matmul, mod.rs:685-688)."""
@@ -479,13 +479,13 @@ class Gpu:
     def split_k(self, a, b, c, partials, slices: int, transposta: bool, colsum: Optional[GpuTensor] = None):
         """ops_split_k (mod.rs:1095-1146)."""
         self._call("rt_gemm_splitk", self._h, TN if transposta else NN, a.handle, b.handle, c.handle,
-                   partials.handle, slices, colsum.handle if colsum else None)
+                   partials.handle, slices, colsum.handle if colsum is not None else None)
 
     def split_k_static(self, a, b, c, slices: int, transposta: bool, colsum: Optional[GpuTensor] = None):
         """split_k with its partial planes in the library's static device
         array: allocates nothing (rt_gemm_splitk_static)."""
         self._call("rt_gemm_splitk_static", self._h, TN if transposta else NN, a.handle, b.handle, c.handle, slices,
-                   colsum.handle if colsum else None)
+                   colsum.handle if colsum is not None else None)
 
     def linear_backward(self, x, delta, w, dx, dw, db=None):
         """dW = Xᵀδ, db = 1ᵀδ, dX = δWᵀ of a Linear layer (one launch when the
@@ -512,7 +512,8 @@ class Gpu:
         self._call("rt_adam", self._h, theta.handle, m.handle, v.handle, g.handle, lr, betas[0], betas[1], eps, t)
 
     def sgd(self, theta, g, lr: float, momentum: float = 0.0, velocity: Optional[GpuTensor] = None):
-        self._call("rt_sgd", self._h, theta.handle, velocity.handle if velocity else None, g.handle, lr, momentum)
+        self._call("rt_sgd", self._h, theta.handle, velocity.handle if velocity is not None else None, g.handle, lr,
+                   momentum)
 
     @staticmethod
     def _handles(ts):

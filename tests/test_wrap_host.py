@@ -97,3 +97,16 @@ def test_tensors_of_the_library_hold_nothing():
 
 def test_null_handles():
     assert G.lib().rt_order_after(None, None) == 2 and G.lib().rt_order_before(None, None) == 2
+
+
+def test_operands_without_elements_are_passed_on():
+    """A tensor of no elements is false, but not absent: the mask of an empty batch, the state of an empty parameter."""
+    gpu, seen = Calls(), []
+    make, t = gpu._call, [gpu.zeros(s) for s in ((0, 8), (0, 5), (8, 5), (0,))]
+    gpu._call = lambda name, *args: seen.append(args) or make(name, *args)
+    gpu.matmul_a_bt(t[1], t[2], t[0], relu_mask_from=t[0])
+    gpu.matmul_at_b(t[1], t[0], t[2], colsum=t[3])
+    gpu.split_k(t[1], t[0], t[2], t[3], 1, True, colsum=t[3])
+    gpu.split_k_static(t[1], t[0], t[2], 1, True, colsum=t[3])
+    gpu.sgd(t[3], t[3], 0.1, 0.9, t[3])
+    assert seen[0][-2] == 16 and all(s[-1] == 16 for s in seen[1:4]) and seen[4][2] == 16
