@@ -621,6 +621,8 @@ def dense_node(x: Var, w: Var, b: Var, relu: bool, checkpoint: bool = False) -> 
         raise ValueError(f"dense: {xv.shape} x {wv.shape} + {bv.shape}")
     if x.tape is not w.tape or w.tape is not b.tape:
         raise ValueError("operands belong to different tapes")
+    if checkpoint and max(k, n) > 1 << 22:  # what the gradient from an 8-bit input takes
+        raise ValueError(f"a checkpointed layer is at most 2^22 wide, got {k} -> {n}")
     a = gpu.empty((m, n))
     gpu.gemm(NN, xv, wv, a, EPI_BIAS_RELU if relu else EPI_BIAS, bv)
     out = Var(x.tape, -1, a)
