@@ -30,6 +30,14 @@ __device__ inline void barrier_lds() {
   asm volatile("s_barrier" ::: "memory");
 }
 
+// Between LDS accesses by which the lanes of one wave pass data to each other: the
+// hardware runs a wave's LDS operations in order, and this keeps the compiler from
+// moving one across (no instruction comes of it).
+__device__ inline void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // s_waitcnt vmcnt(N), leaving the LDS and export counters alone.
 template <int N>
 __device__ inline void wait_vm() {

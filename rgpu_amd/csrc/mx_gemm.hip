@@ -227,6 +227,7 @@ __device__ __forceinline__ void store_rows(const Args& p, const f4 (&acc)[TM][TN
   T* out = static_cast<T*>(p.c) + col;
   static_for<0, TM>([&](auto tc) {
     constexpr int t = decltype(tc)::value;
+    if constexpr (t > 0) rt_dev::wave_lds_order();
 #pragma unroll
     for (int u = 0; u < TN; ++u) {
       f4 v = acc[t][u];
@@ -245,7 +246,7 @@ __device__ __forceinline__ void store_rows(const Args& p, const f4 (&acc)[TM][TN
         *reinterpret_cast<u2*>(at) = u2{h[0] | ((unsigned)h[1] << 16), h[2] | ((unsigned)h[3] << 16)};
       }
     }
-    // The wave alone uses its part: its LDS operations are in order.
+    rt_dev::wave_lds_order();  // the wave alone uses its part
 #pragma unroll
     for (int i = 0; i < 16 / RPI; ++i) {
       const long long row = row0 + 16 * t + i * RPI + rr;
