@@ -167,9 +167,9 @@ int rt_convert_t(rt_ctx* ctx, const rt_buf* src, rt_buf* dst);
  *     last bits of its sums between a product of few rows and one of many.
  *   - RT_TN, A RT_MXFP8 [K, M], B f32, bf16 or f16 [K, N], C f32, no epilogue,
  *     with or without colsum, M and N <= 2^22: the weight gradient from an input
- *     that was saved in 8 bits.  Products are exact (of an f32 B its bits below
- *     2^-133 are dropped; beside an f16 B values of A up to 2^-118 may count as
- *     zeros), additions f32.
+ *     that was saved in 8 bits.  Products are exact but for the bits of A and of
+ *     an f32 B below 2^-133, which are dropped, and for values of A up to 2^-118
+ *     beside an f16 B, which may count as zeros; additions are f32.
  *   - aux of RT_EPI_RELU_MASK may be RT_MXFP8 [M, N] where A and B are f32, bf16
  *     or f16: 1[x > 0] of the finite values x that were converted into it. */
 int rt_gemm(rt_ctx* ctx, rt_layout layout, const rt_buf* a, const rt_buf* b, rt_buf* c,

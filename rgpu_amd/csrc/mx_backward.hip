@@ -3,15 +3,16 @@
 // _f16; and the bias gradient, δ's column sums, from the same tiles.
 //
 // A value of X has four significant bits and a power of two, so it is a bf16
-// without rounding, and an f16 too where its block's scale is from 2^-15 to 2^7.
+// without rounding (from 2^-133 on: the last bits of blocks whose scale is 2^-125
+// or less are lost), and an f16 too where its block's scale is from 2^-15 to 2^7.
 // bf16 δ is multiplied as it stands; f16 δ as well where the scales of the
 // workgroup's part of X span no more than those 22 powers of two: X is multiplied
 // by a power of two that brings them there, C by its inverse (a workgroup looks
 // its scales over first: 1/32 of its codes' bytes).  Else f16 δ goes in as two
 // bf16 planes (11 bits; 262144 rows of 512 x 512 521 us, 160 as it stands); f32 δ
 // as three (24 bits, each plane the next eight by truncation).  So every product
-// is exact, and the sums are f32.  The scale of X varies along the rows that are summed, so it cannot stay
-// outside the product: X is decoded on its way into LDS, where a thread holds 16
+// is exact, and the sums are f32.  The scale of X varies along the rows that are
+// summed, so it cannot stay outside the product: X is decoded on its way into LDS, where a thread holds 16
 // columns of one row, which share a scale.
 //
 // Tiles.  Both operands are contiguous along the output (rows are summed):

@@ -42,3 +42,30 @@ def test_a_batch_of_no_rows(gpu):
     for fmt in (G.MXFP4, G.MXFP8):
         assert gpu.download_f32(gpu.zeros((0, 7), fmt)).shape == (0, 7)
     gpu.sync()
+
+
+@pytest.mark.parametrize("rows,K,N", [(100, 60, 50), (300, 2000, 2048)])
+@pytest.mark.parametrize("dtype,power", [("bf16", 100), ("f32", 100), ("bf16", 0), ("f32", 20), ("f16", 10)])
+def test_gradient_from_the_smallest_values(gpu, rows, K, N, dtype, power):
+    """Values of X whose bits reach below 2^-133, the last of a bf16 (scale bytes 0 to 2): a product keeps those from 2^-133
+    on; beside an f16 gradient values up to 2^-118 may count as zeros."""
+    rng = np.random.default_rng(17)
+    x = (rng.normal(size=(rows, K)) * np.exp2(rng.integers(-130, -117, size=(rows, -(-K // 32))).repeat(32, 1)[:, :K])).astype(
+        np.float32)
+    code, byte, xv = X.quantize(x, G.MXFP8)
+    assert (byte == 0).any() and (byte == 1).any() and (byte == 2).any() and np.any(xv % 2.0 ** -133)
+    q = gpu.upload(X.pack(code, byte, G.MXFP8), G.MXFP8, x.shape)
+    d = np.ldexp(rng.normal(size=(rows, N)), power).astype(np.float32)
+    if dtype == "bf16":
+        d = G.bf16_bits_to_f32(G.f32_to_bf16_bits(d))
+    elif dtype == "f16":
+        d = d.astype(np.float16).astype(np.float32)
+    d64 = d.astype(np.float64)
+    dw = gpu.empty((K, N))
+    gpu.matmul_at_b(q, gpu.upload(d, {"f32": G.F32, "bf16": G.BF16, "f16": G.F16}[dtype]), dw)
+    # the sums as elsewhere; each product short of at most 2^-133 of its factor of X; f32 results that are subnormal
+    # themselves (power 0) are rounded to 2^-149 in each of the sum's steps
+    kept = np.where(np.abs(xv) <= 2.0 ** -118, np.abs(xv), 0) if dtype == "f16" else np.minimum(np.abs(xv), 2.0 ** -133)
+    tol = (3 * rows + 40) * (2.0 ** -23 * (np.abs(xv).T @ np.abs(d64)) + 2.0 ** -149) + kept.T @ np.abs(d64)
+    err = np.abs(gpu.download(dw).astype(np.float64) - xv.T @ d64)
+    assert np.all(err <= tol), (err / tol).max()
