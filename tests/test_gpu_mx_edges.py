@@ -1,4 +1,5 @@
-"""Microscaled tensors at the ends of what they take: batches of no rows, the widest layers."""
+"""Microscaled tensors at the ends of what they take: batches of no rows, the widest layers, every bf16 value, the smallest
+values, tall tensors."""
 import numpy as np
 import pytest
 
@@ -69,3 +70,39 @@ def test_gradient_from_the_smallest_values(gpu, rows, K, N, dtype, power):
     tol = (3 * rows + 40) * (2.0 ** -23 * (np.abs(xv).T @ np.abs(d64)) + 2.0 ** -149) + kept.T @ np.abs(d64)
     err = np.abs(gpu.download(dw).astype(np.float64) - xv.T @ d64)
     assert np.all(err <= tol), (err / tol).max()
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("fmt", [G.MXFP4, G.MXFP8])
+@pytest.mark.parametrize("beside", [None, 0x3F80, 0x4049, 0x0080, 0x7F00])
+def test_every_finite_bf16_value(gpu, fmt, beside, transposed):
+    """All 65280 of them, as they come (blocks of 32 neighbours) or each in a block with one given value."""
+    bits = np.concatenate([np.arange(0x7F80), np.arange(0x8000, 0xFF80)]).astype(np.uint16)
+    if beside is None:
+        bits = bits.reshape(-1, 32 * 8)
+    else:
+        pairs = np.zeros((bits.size, 32), np.uint16)
+        pairs[:, 5], pairs[:, 20] = bits, beside
+        bits = pairs.reshape(-1, 32 * 16)
+    x = G.bf16_bits_to_f32(bits).astype(np.float64)
+    q = gpu.zeros(x.shape, fmt)
+    if transposed:
+        gpu.convert_t(gpu.upload(bits.T.copy(), G.BF16), q)
+    else:
+        gpu.convert(gpu.upload(bits, G.BF16), q)
+    code, byte, _ = X.quantize(x, fmt)
+    assert np.array_equal(gpu.download(q), X.pack(code, byte, fmt))
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("fmt", [G.MXFP4, G.MXFP8])
+@pytest.mark.parametrize("rows,cols", [(4100, 77), (77, 4100), (70001, 5), (5, 70001)])
+def test_tall_and_wide_tensors(gpu, rows, cols, fmt, transposed):
+    x = X.values(np.random.default_rng(rows), rows, cols)
+    t = gpu.upload(x.T.copy() if transposed else x)
+    q, back = gpu.zeros((rows, cols), fmt), gpu.empty((rows, cols))
+    gpu.convert_t(t, q) if transposed else gpu.convert(t, q)
+    gpu.convert(q, back)
+    code, byte, want = X.quantize(x, fmt)
+    assert np.array_equal(gpu.download(q), X.pack(code, byte, fmt))
+    assert np.array_equal(gpu.download(back), want.astype(np.float32))
