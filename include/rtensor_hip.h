@@ -134,7 +134,9 @@ size_t rt_tensor_bytes(rt_dtype dtype, const size_t* shape, int rank);
  * in the reference): a block's scale is the least power of two, from 2^-127 on,
  * at which its largest finite magnitude does not pass 6 (RT_MXFP4) or 448
  * (RT_MXFP8), and its elements are rounded to nearest, ties to even: each is
- * within half a step of its value, and none saturates.  An infinity or NaN makes
+ * within half a step of its value, and none saturates (the OCP microscaling
+ * conversion takes half that scale for a maximum of more than 1.5, or 1.75, times
+ * a power of two, and lets it saturate).  An infinity or NaN makes
  * its RT_MXFP4 block NaN; in RT_MXFP8 it alone becomes NaN.  In RT_MXFP8 a value
  * that rounds to zero is stored as code 0x80 if it was positive and 0 if not, so
  * that 1[x > 0] of finite values can be read from the codes exactly.  Back, each

@@ -12,17 +12,17 @@
 // bf16 planes (11 bits; 262144 rows of 512 x 512 521 us, 160 as it stands); f32 δ
 // as three (24 bits, each plane the next eight by truncation).  So every product
 // is exact, and the sums are f32.  The scale of X varies along the rows that are
-// summed, so it cannot stay outside the product: X is decoded on its way into LDS, where a thread holds 16
-// columns of one row, which share a scale.
+// summed, so it cannot stay outside the product: X is decoded on its way into LDS,
+// where a thread holds 16 columns of one row, which share a scale.
 //
 // Tiles.  Both operands are contiguous along the output (rows are summed):
 // LDS holds them by rows and fragments come out by transposed reads
 // (ds_read_b64_tr_b16).  Few output tiles over many rows are cut into slices of
 // rows, whose f32 planes splitk_reduce adds in slice order.
 //
-// Measured: 8192 rows, 4096 x 4096, bf16 with the bias gradient 246 us (1.12
-// PFLOP/s; a library product of 8192^3 1.21 on the same card); 262144 rows of 512 x
-// 512 158 (2.6 TB/s); 2048 rows, 1024 x 1024, f32 33 with the sum of its slices.
+// Measured: 8192 rows, 4096 x 4096, bf16 with the bias gradient 246-274 us (1.0 to
+// 1.12 PFLOP/s; a library product of 8192^3 1.21); 262144 rows of 512 x 512 158-175
+// (2.3-2.6 TB/s); 2048 rows, 1024 x 1024, f32 33 with the sum of its slices.
 
 #include <algorithm>
 #include <type_traits>

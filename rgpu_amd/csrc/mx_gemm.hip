@@ -35,8 +35,9 @@
 // the end of A or B are zeros by the buffer descriptors' range check; K is whole
 // steps by the layout.
 //
-// Measured: 4 bits, 8192 x 16384, K 4096, bf16 C, 298 us (3.7 PFLOP/s; its 268 MB
-// of C at the copy rate take 52); 8 bits, 8192 x 4096, K 4096, 193-241 us (1.1 to
+// Measured: 4 bits, 8192 x 16384, K 4096, bf16 C, 298-342 us (3.2-3.7 PFLOP/s, of
+// 8.9 that the instruction alone reaches: matrix units busy 38%; the 268 MB of C at
+// the copy rate take 52); 8 bits, 8192 x 4096, K 4096, 193-241 us (1.1 to
 // 1.4 PFLOP/s); one row by 4096 x 4096 weights 4.4 us, of which a launch is 3.2.
 
 #include <algorithm>
