@@ -332,8 +332,7 @@ def prepare(case, seed):
             out.update(rows=empty(rows, dout, dtype=t), dw=empty(e, din, dout), db=empty(e, dout),
                        dx=empty(n, din, dtype=t))
         elif case["mode"] == "serve":
-            # What is added up over a token's choices is held in f32 until then.
-            s["h"], s["o"] = empty(rows, dout, dtype=t), empty(rows, din)
+            s["h"], s["o"] = empty(rows, dout, dtype=t), empty(rows, din, dtype=t)
             out["y"] = empty(n, din, dtype=t)
         else:
             s["do"], s["dh"], s["dxr"] = empty(rows, din), empty(rows, dout), empty(rows, din)
