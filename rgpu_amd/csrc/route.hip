@@ -349,17 +349,22 @@ __device__ bool route_fast(const RouteArgs& p, long long token, int lane, RouteR
     }
   }
   // The k-th greatest of the token's values m (of different ones, so never above
-  // the k-th of all c where m are among them), and the candidates above it.
+  // the k-th of all c where m are some of them), and the candidates above it.  Fewer
+  // than k different numbers say nothing of the k-th of all c, unless m are all c.
   float least = 0.0f;
   unsigned count = 0, upto = 0, all = 0;  // candidates of this lane, with those of the lanes before it, of the token
   auto choose = [&](auto nc, const float* m) {
     float kth = INFINITY;
+    bool short_of_k = false;
     for (int r = 0; r < p.k; ++r) {
       float best = -INFINITY;
 #pragma unroll
       for (int v = 0; v < decltype(nc)::value; ++v) best = fmaxf(best, m[v] < kth ? m[v] : -INFINITY);
       best = lanes_max<LANES>(best);
-      if (best == -INFINITY) break;  // the wave's other tokens may go on
+      if (best == -INFINITY) {  // the wave's other tokens may go on
+        short_of_k = decltype(nc)::value < VPL;
+        break;
+      }
       kth = best;
     }
     least = kth - far(kth);
@@ -372,7 +377,7 @@ __device__ bool route_fast(const RouteArgs& p, long long token, int lane, RouteR
     upto += dpp<0x114>(upto);
     upto += dpp<0x118>(upto);
     all = (unsigned)__shfl((int)upto, (threadIdx.x & 48) + 15, 64);
-    return !(fabsf(kth) < INFINITY) || all > LANES || all < (unsigned)p.k;
+    return short_of_k || !(fabsf(kth) < INFINITY) || all > LANES || all < (unsigned)p.k;
   };
   // First by the greatest of each half of a lane's values: the k-th of those 32 is a
   // little low, and seldom so low that 16 lanes do not hold what is above it.
