@@ -441,19 +441,28 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
 //   softmax: dx_e = s_e (ds_e [e chosen] - sum_j s_j ds_j), whose second term
 //            is 0 when renormalised (the weights are then a softmax of the
 //            chosen logits alone).
+// So a chosen expert's is s_j (g_j - sum_i w_i g_i), of weights w that add up to
+// 1 with those of g = 0 (the experts that softmax did not choose).  Where one
+// weight is nearly 1 that is a small difference of large numbers, so with
+// m the chosen of the greatest logit it is added up as
+//   s_j (g_j U + sum_i w_i (g_m - g_i) + (g_j - g_m) sum_i w_i),
+// i over the chosen and U what the others' weights add up to; 1 - sigmoid(x) is
+// likewise exp(-x) sigmoid(x).
 // The chosen s are held in 64 bits: a bias or the groups may choose experts whose
 // scores are all below what 32 bits hold, and their quotients are still weights.
 template <int DT, int LANES, int VPL>
 __global__ __launch_bounds__(256) void route_grad_kernel(RouteArgs p) {
   constexpr int ROWS = 256 / LANES, T = kMaxChoices / LANES;
-  __shared__ float dx[ROWS][LANES * VPL];
-  __shared__ float add[ROWS][kMaxChoices];
-  __shared__ unsigned at[ROWS][kMaxChoices];
-  const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
+  __shared__ unsigned slots[ROWS][LANES * VPL];  // of each expert: its first choice, then its gradient
+  const int lane = threadIdx.x % LANES;
+  unsigned* const of = slots[threadIdx.x / LANES];
+  const bool whole = !p.sigmoid && !p.renorm;  // weights of all experts add up to 1, not of the chosen
   for (long long t0 = (long long)blockIdx.x * ROWS; t0 < p.tokens; t0 += (long long)gridDim.x * ROWS) {
-  const long long token = t0 + slot;
+  const long long token = t0 + threadIdx.x / LANES;
   const long long row = min(token, p.tokens - 1) * p.experts, ch = min(token, p.tokens - 1) * p.k;
   const int E = p.experts;
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) of[v * LANES + lane] = kMaxChoices;
   float x[VPL], top = -INFINITY, total = 0.0f;
   if (!p.sigmoid) {
 #pragma unroll
@@ -472,51 +481,98 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteArgs p) {
     total = lanes_sum<LANES>(total);
     if (total == 0.0f) total = 1.0f;
   }
-  double s[T], g[T], z = 0.0, gs = 0.0;
+  // The choices: score, 1 - score (sigmoid), gradient; the logit and the gradient of the greatest.
+  double s[T], rest1[T], g[T];
   unsigned id[T];
+  float most = -INFINITY, gm = 0.0f;
+  auto greater = [&](float l, float gl) {  // of equal logits the greater gradient: the same in every lane
+    const bool other = l > most || (l == most && gl > gm);
+    most = other ? l : most;
+    gm = other ? gl : gm;
+  };
+  rt_dev::wave_lds_order();
 #pragma unroll
   for (int t = 0; t < T; ++t) {
     const int j = t * LANES + lane;
     s[t] = g[t] = 0.0;
+    rest1[t] = 1.0;
     id[t] = 0xffffffffu;
     if (j < p.k) {
       id[t] = p.ids[ch + j];
       if (id[t] < (unsigned)E) {
-        const double l = (double)rt_dev::load1<DT>(p.logits, row + id[t]);
-        s[t] = p.sigmoid ? sigmoid64(l) : exp(l - (double)top) / (double)total;
-        g[t] = (double)p.dweights[ch + j];
+        const float l = rt_dev::load1<DT>(p.logits, row + id[t]), gl = p.dweights[ch + j];
+        if (p.sigmoid) {
+          const double power = exp(-(double)l);
+          s[t] = 1.0 / (1.0 + power);
+          if (power < INFINITY) rest1[t] = power * s[t];
+        } else {
+          s[t] = exp((double)l - (double)top) / (double)total;
+        }
+        g[t] = (double)gl;
+        greater(l, gl);
+        atomicMin(&of[id[t]], (unsigned)j);
       }
     }
-    z += s[t];
+  }
+  over_lanes<LANES>([&](auto from) {
+    const float l = __uint_as_float(from(__float_as_uint(most))), gl = __uint_as_float(from(__float_as_uint(gm)));
+    greater(l, gl);
+  });
+  rt_dev::wave_lds_order();
+  bool first[T], again = false;  // whether a choice is the first of its expert (a program's own may repeat one)
+  double z = 0.0, gs = 0.0, apart = 0.0, others = 0.0;
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    first[t] = id[t] < (unsigned)E && of[id[t]] == (unsigned)(t * LANES + lane);
+    again |= id[t] < (unsigned)E && !first[t];
+    const bool once = !whole || first[t];
+    z += once ? s[t] : 0.0;
+    apart += s[t] * ((once ? (double)gm : 0.0) - g[t]);
     gs += s[t] * g[t];
   }
   z = lanes_sum<LANES>(z);
-  gs = lanes_sum<LANES>(gs);
-  const bool none = z == 0.0;  // no chosen score: the weights were zeros
-  const double f = !p.renorm ? (double)p.scale : none ? 0.0 : (double)p.scale / z;
-  const double mean = p.renorm && !none ? gs / z : 0.0;
+  apart = lanes_sum<LANES>(apart);
+  float rest = 0.0f;  // of the experts that were not chosen: -sum_j s_j ds_j
+  if (whole) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) sum += of[v * LANES + lane] == kMaxChoices ? x[v] : 0.0f;
+    others = (double)lanes_sum<LANES>(sum) / (double)total;
+    rest = -p.scale * (float)lanes_sum<LANES>(gs);
+  }
+  rt_dev::wave_lds_order();
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) of[v * LANES + lane] = __float_as_uint(rest == 0.0f ? 0.0f : rest * (x[v] / total));
+  rt_dev::wave_lds_order();
+  float add[T];
 #pragma unroll
   for (int t = 0; t < T; ++t) {
-    const int j = t * LANES + lane;
-    if (j < kMaxChoices) {
-      const double d = s[t] * f * (g[t] - mean);
-      add[slot][j] = (float)(p.sigmoid ? d * (1.0 - s[t]) : d);
-      at[slot][j] = id[t];
+    add[t] = 0.0f;
+    if (t * LANES + lane >= p.k) continue;
+    double d = g[t], w = s[t];
+    if (p.renorm) {
+      w = z == 0.0 ? 0.0 : s[t] / z;  // no chosen score: the weights were zeros
+      d = z == 0.0 ? 0.0 : apart / z + (g[t] - (double)gm);
+    } else if (whole && first[t]) {
+      d = g[t] * others + (apart + (g[t] - (double)gm) * z);
     }
+    add[t] = (float)(w * (double)p.scale * d * rest1[t]);
+    if (first[t]) of[id[t]] = __float_as_uint(add[t]);
   }
-  const float rest = p.sigmoid || p.renorm ? 0.0f : -p.scale * (float)gs;  // -sum_j s_j ds_j
+  rt_dev::wave_lds_order();
+  if (__any(again)) {
 #pragma unroll
-  for (int v = 0; v < VPL; ++v) dx[slot][v * LANES + lane] = rest == 0.0f ? 0.0f : rest * (x[v] / total);
-  rt_dev::wave_lds_order();
-  for (int j = 0; j < p.k; ++j) {  // each lane the experts that are its own
-    const unsigned e = at[slot][j];
-    if (e < (unsigned)E && e % LANES == (unsigned)lane) dx[slot][e] += add[slot][j];
+    for (int t = 0; t < T; ++t)
+      for (int l = 0; l < LANES; ++l) {  // in their order
+        if (lane == l && id[t] < (unsigned)E && !first[t])
+          of[id[t]] = __float_as_uint(__uint_as_float(of[id[t]]) + add[t]);
+        rt_dev::wave_lds_order();
+      }
   }
-  rt_dev::wave_lds_order();
 #pragma unroll
   for (int v = 0; v < VPL; ++v) {
     const int e = v * LANES + lane;
-    if (e < E && token < p.tokens) rt_dev::store1<DT>(p.dlogits, row + e, dx[slot][e]);
+    if (e < E && token < p.tokens) rt_dev::store1<DT>(p.dlogits, row + e, __uint_as_float(of[e]));
   }
   rt_dev::wave_lds_order();
   }

@@ -1,4 +1,5 @@
-"""Routing where its 32-bit steps could decide otherwise than 64 bits."""
+"""Routing where its 32-bit steps could decide otherwise than 64 bits, and its gradient where it is a small difference of large
+terms."""
 import numpy as np
 import pytest
 
@@ -57,3 +58,86 @@ def test_route_of_more_choices_than_columns(gpu, kind, k):
     w /= w.sum(axis=1, keepdims=True)
     rows = same.all(axis=1)
     assert rows.mean() > 0.99 and np.all(abs(gpu.download(weights) - w)[rows] <= 2.0 ** -23 * w[rows])
+
+
+def gradient(x, ids, g, score, renormalise, scale):
+    """(dx, what its terms add up to without their signs), from sums that hold no difference of nearly equal numbers but
+    those of the given g: with e the powers, T their sum over all experts (or over the chosen, if renormalised),
+    g_j - sum_i w_i g_i = (g_j sum of the e not chosen + sum_i e_i (g_j - g_i)) / T; 1 - sigmoid(z) = sigmoid(-z)."""
+    x, g = x.astype(np.float64), g.astype(np.float64)
+    e = T.scores(x, "sigmoid") if score == "sigmoid" else np.exp(x - x.max(axis=1, keepdims=True))
+    ej = np.take_along_axis(e, ids, axis=1)
+    left = e.copy()
+    np.put_along_axis(left, ids, 0, axis=1)
+    left = left.sum(axis=1, keepdims=True)
+    apart = g[:, :, None] - g[:, None, :]
+    if renormalise:
+        total = ej.sum(axis=1, keepdims=True)
+        d, size = ej * (ej[:, None] * apart).sum(axis=2) / total ** 2, ej * (ej[:, None] * abs(apart)).sum(axis=2) / total ** 2
+    elif score == "softmax":
+        total = ej.sum(axis=1, keepdims=True) + left
+        d = ej * (g * left + (ej[:, None] * apart).sum(axis=2)) / total ** 2
+        size = ej * (abs(g) * left + (ej[:, None] * abs(apart)).sum(axis=2)) / total ** 2
+    else:
+        d, size = ej * g, ej * abs(g)
+    if score == "sigmoid":
+        rest = T.scores(-np.take_along_axis(x, ids, axis=1), "sigmoid")
+        d, size = d * rest, size * rest
+    dx, big = np.zeros_like(e), np.zeros_like(e)
+    if score == "softmax" and not renormalise:
+        dx, big = -e * (ej * g).sum(axis=1, keepdims=True) / total ** 2, e * (ej * abs(g)).sum(axis=1, keepdims=True) / total ** 2
+    np.put_along_axis(dx, ids, d, axis=1)
+    np.put_along_axis(big, ids, size, axis=1)
+    return scale * dx, scale * big
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalise", [True, False])
+@pytest.mark.parametrize("experts,k", [(2, 1), (8, 1), (8, 2), (8, 8), (64, 4), (256, 8), (300, 20), (1024, 64)])
+@pytest.mark.parametrize("gap", [0, 8, 12, 17, 30, 60])
+def test_route_backward_of_a_confident_router(gpu, score, renormalise, experts, k, gap):
+    """One logit `gap` above the others: the chosen ones' gradients are as small as what is left of 1, and as exact."""
+    rng = np.random.default_rng(experts + k + gap)
+    n = 40
+    x = (rng.normal(size=(n, experts)) * 0.5).astype(np.float32)
+    x[np.arange(n), rng.integers(0, experts, n)] += gap
+    if score == "sigmoid" and renormalise:
+        x -= np.float32(gap)  # scores from 0.5 down
+    ids = T.route(x, k, score)[0]
+    g = rng.normal(size=(n, k)).astype(np.float32)
+    g[::3] = g[::3, :1]  # one gradient for all: nothing but what the others' scores leave
+    dx = gpu.empty((n, experts))
+    gpu.route_backward(gpu.upload(x), T.words(gpu, ids), gpu.upload(g), dx, score=score, renormalise=renormalise, scale=2.5)
+    want, size = gradient(x, ids, g, score, renormalise, 2.5)
+    # f32 powers: the difference from the greatest logit rounded (half a step of at most gap + 4), two steps of their
+    # own, at most 22 additions: once in what was not chosen, twice in the sum (there without the gap, whose terms are as
+    # much smaller); a dozen roundings beside
+    err = (gap + 3 * (4 + 4 + 22) + 12) * 2.0 ** -24 * size
+    assert np.all(abs(gpu.download(dx) - want) <= err + T.LEAST[G.F32])
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalise", [True, False])
+def test_route_backward_of_an_expert_named_twice(gpu, score, renormalise):
+    """A program's own choice may name an expert more than once: each time counts."""
+    rng = np.random.default_rng(0)
+    x, g = rng.normal(size=(30, 20)).astype(np.float32), rng.normal(size=(30, 5)).astype(np.float32)
+    ids = rng.integers(0, 4, (30, 5))
+    ids[::5, 1] = G.PADDING
+    dx = gpu.empty((30, 20))
+    gpu.route_backward(gpu.upload(x), T.words(gpu, ids), gpu.upload(g), dx, score=score, renormalise=renormalise, scale=1.5)
+    s = T.scores(x, score)
+    want, size = np.zeros((30, 20)), np.zeros((30, 20))
+    for t in range(30):
+        on = [j for j in range(5) if ids[t, j] < 20]
+        sj = s[t, ids[t, on]]
+        z = sj.sum() if renormalise else 1.0
+        ds, big = np.zeros(20), np.zeros(20)  # of the scores
+        np.add.at(ds, ids[t, on], 1.5 * g[t, on] / z - (1.5 * (g[t, on] * sj).sum() / z ** 2 if renormalise else 0))
+        np.add.at(big, ids[t, on], 1.5 * abs(g[t, on]) / z + (1.5 * (abs(g[t, on]) * sj).sum() / z ** 2 if renormalise else 0))
+        if score == "sigmoid":
+            want[t], size[t] = s[t] * (1 - s[t]) * ds, s[t] * big
+        else:
+            want[t], size[t] = s[t] * (ds - (s[t] * ds).sum()), s[t] * (big + (s[t] * big).sum())
+    # as without repetitions: powers and their sum to a few steps, a dozen roundings, at most 5 f32 additions
+    assert np.all(abs(gpu.download(dx) - want) <= 50 * 2.0 ** -24 * size + T.LEAST[G.F32])
