@@ -94,6 +94,12 @@ __device__ inline float lanes_max(float v) {
 
 __device__ inline double sigmoid64(double x) { return 1.0 / (1.0 + exp(-x)); }
 
+// Divided before it is scaled: the reciprocal of a sum below 2^-1024 is infinite.
+__device__ inline float weight_of(const RouteArgs& p, double score, double sum) {
+  const double w = !p.renorm ? score : sum == 0.0 ? 0.0 : score / sum;
+  return (float)(w * (double)p.scale);
+}
+
 // A token's LDS: its group's c (kept groups only) and its choices.
 template <int LANES, int VPL>
 struct RouteRow {
@@ -210,13 +216,12 @@ __device__ void route_exact(const RouteArgs& p, long long token, int lane, Route
     sum += s[t];
   }
   sum = lanes_sum<LANES>(sum);
-  const double f = p.renorm ? (sum == 0.0 ? 0.0 : (double)p.scale / sum) : (double)p.scale;
 #pragma unroll
   for (int t = 0; t < kMaxChoices / LANES; ++t) {
     const int j = t * LANES + lane;
     if (j < p.k && token < p.tokens) {
       p.ids[token * p.k + j] = lds.chosen[j];
-      p.weights[token * p.k + j] = (float)(s[t] * f);
+      p.weights[token * p.k + j] = weight_of(p, s[t], sum);
     }
   }
 }
@@ -411,10 +416,9 @@ __device__ bool route_fast(const RouteArgs& p, long long token, int lane, RouteR
   });
   const bool chosen = in && rank < p.k;
   const double sum = lanes_sum<LANES>(chosen ? score : 0.0);
-  const double f = p.renorm ? (sum == 0.0 ? 0.0 : (double)p.scale / sum) : (double)p.scale;
   if (chosen && token < p.tokens) {
     p.ids[token * p.k + rank] = e;
-    p.weights[token * p.k + rank] = (float)(score * f);
+    p.weights[token * p.k + rank] = weight_of(p, score, sum);
   }
   return true;
 }

@@ -141,3 +141,29 @@ def test_route_backward_of_an_expert_named_twice(gpu, score, renormalise):
             want[t], size[t] = s[t] * (ds - (s[t] * ds).sum()), s[t] * (big + (s[t] * big).sum())
     # as without repetitions: powers and their sum to a few steps, a dozen roundings, at most 5 f32 additions
     assert np.all(abs(gpu.download(dx) - want) <= 50 * 2.0 ** -24 * size + T.LEAST[G.F32])
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,k", [(8, 1), (64, 3), (100, 20), (600, 4)])
+def test_weights_of_scores_whose_reciprocal_is_infinite(gpu, score, experts, k):
+    """A bias takes out the experts with the great scores; those left are below 2^-1022, and weigh `scale` together."""
+    rng = np.random.default_rng(experts)
+    low = (-709.7, -709.0) if score == "sigmoid" else (-718.0, -709.0)
+    x = rng.uniform(*low, (5, experts)).astype(np.float32)
+    x[:, :experts // 2] = 0
+    bias = np.zeros(experts, np.float32)
+    bias[:experts // 2] = -np.inf
+    ids, weights, dx = gpu.empty((5, k), G.U32), gpu.empty((5, k)), gpu.empty((5, experts))
+    gpu.route(gpu.upload(x), ids, weights, gpu.upload(bias), score=score, scale=2.5)
+    got = gpu.download(ids).astype(np.int64)
+    assert got.min() >= experts // 2
+    z = np.take_along_axis(x, got, 1).astype(np.float64)  # 1 / (1 + e^-z) is e^z here, to 300 places
+    w = np.exp(z - z.max(axis=1, keepdims=True))
+    w *= 2.5 / w.sum(axis=1, keepdims=True)
+    # one rounding; a score is a whole number of 2^-1074, at least 2^36 of them
+    assert np.all(abs(gpu.download(weights) - w) <= 2.0 ** -23 * w)
+    g = rng.normal(size=(5, k)).astype(np.float32)
+    gpu.route_backward(gpu.upload(x), ids, gpu.upload(g), dx, score=score, scale=2.5)
+    want = np.zeros((5, experts))
+    np.put_along_axis(want, got, w * (g - (w / 2.5 * g).sum(axis=1, keepdims=True)), axis=1)
+    assert np.all(abs(gpu.download(dx) - want) <= 2.0 ** -22 * 2.5 * abs(g).max())
