@@ -727,12 +727,10 @@ class Embedding:
 
     def input(self, ids) -> GpuTensor:
         """Tokens on the device."""
-        return ids if isinstance(ids, GpuTensor) else upload_ids(self.w.gpu, ids)
+        return _tokens(self.w.gpu, ids)
 
     def out_shape(self, ids: GpuTensor) -> Shape:
-        if ids.dtype != U32 or len(ids.shape) not in (1, 2):
-            raise ValueError(f"an embedding takes tokens [rows] or [rows, places], got {ids.shape}")
-        return (ids.shape[0], _numel(ids.shape[1:]) * self.w.shape[1])
+        return _embedded_shape(ids, self.w.shape[1])
 
     def forward(self, x: Var) -> Var:
         gpu, ids, scale = x.gpu, x.value, self.scale
@@ -753,6 +751,16 @@ class Embedding:
 
     def describe(self) -> str:
         return f"Embedding({self.w.shape[0]} x {self.w.shape[1]})"
+
+
+def _tokens(gpu: Gpu, ids) -> GpuTensor:
+    return ids if isinstance(ids, GpuTensor) else upload_ids(gpu, ids)
+
+
+def _embedded_shape(ids: GpuTensor, dim: int) -> Shape:
+    if ids.dtype != U32 or len(ids.shape) not in (1, 2):
+        raise ValueError(f"an embedding takes tokens [rows] or [rows, places], got {ids.shape}")
+    return (ids.shape[0], _numel(ids.shape[1:]) * dim)
 
 
 class Dropout:
@@ -949,9 +957,8 @@ class QuantizedSequential:
             if isinstance(layer, Dropout):
                 continue
             if isinstance(layer, Embedding) and i == 0:
-                table = layer.w.gpu.empty(layer.w.shape, BF16)
-                layer.w.gpu.convert(layer.w.tensor, table)
-                self.table, self._embedding = table, layer
+                self.table, self._scale = layer.w.gpu.empty(layer.w.shape, BF16), layer.scale
+                layer.w.gpu.convert(layer.w.tensor, self.table)
                 continue
             if not all(hasattr(layer, name) for name in ("w", "b", "activation")):
                 raise ValueError(f"layer {i}: {layer.describe()} is not served in 4 bits")
@@ -969,9 +976,9 @@ class QuantizedSequential:
         begins with an Embedding) to f32 [rows, units]."""
         gpu = self.layers[0][0].gpu
         if self.table is not None:
-            ids = self._embedding.input(x)
-            x = gpu.empty(self._embedding.out_shape(ids), BF16)
-            gpu.embed(self.table, ids, x, self._embedding.scale)
+            ids = _tokens(gpu, x)
+            x = gpu.empty(_embedded_shape(ids, self.table.shape[1]), BF16)
+            gpu.embed(self.table, ids, x, self._scale)
         x = _as_device(gpu, x)
         for i, (w4, b, activation) in enumerate(self.layers):
             kind, slope = _activation(activation)
