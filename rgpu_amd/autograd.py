@@ -922,7 +922,7 @@ class Sequential:
         for a first Embedding may be a host array."""
         first = self.layers[0]
         gpu = first.w.gpu if hasattr(first, "w") else first.gpu
-        x = first.input(x) if hasattr(first, "input") else x
+        x = first.input(x) if isinstance(first, Embedding) else x
         return self.forward(constant(Tape(gpu, training=False), x)).value
 
     def params(self) -> List[Param]:
