@@ -31,6 +31,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 import os
 from typing import List, Optional, Sequence
 
@@ -596,7 +597,8 @@ class Gpu:
         (a whole number of 65536ths), the mask a function of (seed, draw) and
         the element's number: the same call on the gradient is the backward
         pass.  y may be x.  Take another draw for each use."""
-        self._call("rt_dropout", self._h, x.handle, y.handle, p, seed & _U64, draw & _U64)
+        self._call("rt_dropout", self._h, x.handle, y.handle, p, operator.index(seed) & _U64,
+                   operator.index(draw) & _U64)
 
     def embed(self, table, ids, out, scale: float = 1.0):
         """out = scale * table[ids]; rows of zeros for ``PADDING``."""
