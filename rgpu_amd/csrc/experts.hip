@@ -777,7 +777,9 @@ hipError_t experts_launch(hipStream_t s, const ExpertArgs& args, float* rows) {
       return experts_tiles<RT_NN, 4, 64>(s, p, experts_few_kernel<DT, 64>, 512);
     }
   }
-  if (LAYOUT != RT_TN && mean <= 32) return experts_regs<DT, LAYOUT, 32, 64, 1, 4>(s, p);
+  if constexpr (LAYOUT != RT_TN) {
+    if (mean <= 32) return experts_regs<DT, LAYOUT, 32, 64, 1, 4>(s, p);
+  }
   if constexpr (DT != RT_F32) {
     // Tiles of C; an expert's rows leave half a tile over on average.
     auto tiles = [&](long long b) {
@@ -795,15 +797,23 @@ hipError_t experts_launch(hipStream_t s, const ExpertArgs& args, float* rows) {
         return experts_dma<DT, LAYOUT, 256, 256, 2, 4, 2>(s, p);
       // Where a 128x128 tile has a CU to itself, four stages (8 experts 1024 x
       // 1024 over 1024 rows NN 17.2 us, 18.7 in two; over 4096 34.2 and 26.3).
-      if (LAYOUT != RT_TN && tiles(128) <= 256) return experts_dma<DT, LAYOUT, 128, 128, 2, 2, 4>(s, p);
+      if constexpr (LAYOUT != RT_TN) {
+        if (tiles(128) <= 256) return experts_dma<DT, LAYOUT, 128, 128, 2, 2, 4>(s, p);
+      }
       return experts_dma<DT, LAYOUT, 128, 128, 2, 2, 2>(s, p);
     }
     // Through registers smaller tiles, where few, keep more loads on their way (5
     // experts 1003 x 777 over 3000 rows NN 28.7 us, 46.0 in 128x128 tiles; 8 of
     // 1001 x 2003 over 8000 122 and 104), TN, which is short here, always (35.5 and 54.0).
-    if (LAYOUT == RT_TN || tiles(128) <= 256) return experts_regs<DT, LAYOUT, 64, 64, 2, 2>(s, p);
+    if constexpr (LAYOUT == RT_TN) {
+      return experts_regs<DT, LAYOUT, 64, 64, 2, 2>(s, p);
+    } else {
+      if (tiles(128) <= 256) return experts_regs<DT, LAYOUT, 64, 64, 2, 2>(s, p);
+      return experts_regs<DT, LAYOUT, 128, 128, 2, 2>(s, p);
+    }
+  } else {
+    return experts_regs<DT, LAYOUT, 128, 128, 2, 2>(s, p);
   }
-  return experts_regs<DT, LAYOUT, 128, 128, 2, 2>(s, p);
 }
 
 // Slices of the TN product's rows: where its tiles leave half the chip idle (f32:
