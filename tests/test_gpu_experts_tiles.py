@@ -190,3 +190,45 @@ def test_few_rows(gpu, dtype, tokens, k, K, experts, N):
     for out in {G.F32, dtype}:
         for ordered, epi in ((True, G.EPI_NONE), (False, G.EPI_BIAS), (True, G.EPI_BIAS_RELU), (False, G.EPI_RELU_MASK)):
             check_nn(c, out, ordered, epi)
+
+
+@pytest.mark.parametrize("dtype", T.TYPES, ids=NAMES)
+@pytest.mark.parametrize("rows", [50, 300])
+@pytest.mark.parametrize("wide", [72, 131])
+def test_products_of_no_inner_dimension(gpu, dtype, rows, wide):
+    off = T.words(gpu, [0, rows // 3, rows - 2])
+    bias = np.random.default_rng(rows).normal(size=(2, wide)).astype(np.float32)
+    c = gpu.upload(np.full((rows, wide), 7, np.float32))
+    gpu.experts_gemm(G.NN, gpu.empty((rows, 0), dtype), gpu.empty((2, 0, wide), dtype), c, off, None, G.EPI_BIAS, gpu.upload(bias))
+    want = np.full((rows, wide), 7, np.float32)
+    want[:rows // 3], want[rows // 3:rows - 2] = bias
+    assert np.array_equal(gpu.download(c), want)
+    c = gpu.upload(np.full((rows, wide), 7, np.float32))
+    gpu.experts_gemm(G.NT, gpu.empty((rows, 0), dtype), gpu.empty((2, wide, 0), dtype), c, off)
+    want[:rows - 2] = 0
+    assert np.array_equal(gpu.download(c), want)
+
+
+# Matrices of more than 2^21 a side, f32: 128x128 register tiles, mean above 32.  Whole numbers, so sums are exact.
+@pytest.mark.parametrize("ordered", [True, False])
+def test_f32_matrices_of_more_than_2_21_a_side(gpu, ordered):
+    rows, long = 74, (1 << 21) + 5
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(3)
+    whole = lambda *s: torch.randint(-1, 2, s, generator=gen, device="cuda").float()  # noqa: E731
+    held = lambda t: gpu.wrap(t.data_ptr(), tuple(t.shape), G.F32, owner=t)  # noqa: E731
+    order = torch.randperm(rows, generator=gen, device="cuda")
+    off, d_order = T.words(gpu, [0, 40, rows - 1]), T.words(gpu, order.cpu().numpy()) if ordered else None
+    a, d, w, wt = whole(rows, long), whole(rows, 6), whole(2, long, 6), whole(2, 6, long)
+    pick = a[order] if ordered else a
+    c, dx, dw = (torch.full(s, 7.0, device="cuda") for s in ((rows, 6), (rows, 6), (2, long, 6)))
+    torch.cuda.synchronize()
+    gpu.experts_gemm(G.NN, held(a), held(w), held(c), off, d_order)
+    gpu.experts_gemm(G.NT, held(a), held(wt), held(dx), off)
+    gpu.experts_gemm(G.TN, held(a), held(d), held(dw), off, d_order)
+    gpu.sync()
+    for e, (s, t) in enumerate(((0, 40), (40, rows - 1))):
+        assert torch.equal(c[s:t], (pick[s:t].double() @ w[e].double()).float())
+        assert torch.equal(dx[s:t], (a[s:t].double() @ wt[e].double().T.contiguous()).float())
+        assert torch.equal(dw[e], (pick[s:t].double().T.contiguous() @ d[s:t].double()).float())
+    assert bool((c[rows - 1] == 7).all()) and bool((dx[rows - 1] == 7).all())
