@@ -714,13 +714,15 @@ __global__ __launch_bounds__(256) void pad_kernel(PadArgs t) {
 }
 
 // Whether a TN product goes through padded copies: where it has rows enough for
-// them, and work (f16, us with copies and without: 8 experts 1001 x 2003 over 8000
-// rows 81 and 153, 16 of 515 x 1027 over 32768 124 and 220, 5 of 1003 x 777 over
-// 3000 32.7 and 35.5; 4 over 1200 22.6 and 18.1, 64 of 513 x 1025 over 8192, 128
-// rows an expert, 78 and 76).
+// them, and work.  f16, us with copies and without, by multiply-adds: 2^29.9 (2
+// experts 1003 x 333 over 3000 rows) 27.1 and 26.4, 2^30.0 (5 of 1003 x 777 over
+// 1400) 25.1 and 23.8, 2^30.4 (over 1800) 27.4 and 27.9, 2^30.5 (1 of 1003 x 1001
+// over 1500) 28.5 and 30.5, 2^30.7 (16 of 333 x 333 over 16000) 39.7 and 48.9,
+// 2^31.0 (8 of 515 x 1027 over 4000) 31.5 and 37.4, 2^33.9 (8 of 1001 x 2003 over
+// 8000) 81 and 153; of 128 rows an expert (64 of 513 x 1025 over 8192) 78 and 76.
 bool pads(const ExpertArgs& p, int dtype) {
   if (dtype == RT_F32 || dma_ok<RT_TN>(p) || p.n / p.experts < 256) return false;
-  return (double)p.n * p.K * p.N >= 0x1p31 && p.n * (std::max(p.K, p.N) + 7LL) * 2 < 1LL << 31;
+  return (double)p.n * p.K * p.N >= 0x1.4p30 && p.n * (std::max(p.K, p.N) + 7LL) * 2 < 1LL << 31;
 }
 
 // f32 products of many rows go to the split kernel of gemm_f32.hip, whose tiles

@@ -146,11 +146,12 @@ def test_forward_and_input_gradient_in_16_bits(gpu, dtype, tokens, k, experts, w
     check_nt(Case(gpu, dtype, tokens, k, experts, wide, deep), out)
 
 
-# 256x256 tiles where 256 of them (9 x 5 x 6; 2 slices of 130), else 128x128: whole, in four slices (120 tiles of 128x128), and
-# of padded copies (odd widths, 2^31 multiply-adds) in 25 slices.
+# 256x256 tiles where 256 of them (9 x 5 x 6; 2 slices of 130), else 128x128: whole, in four slices (120 tiles), and
+# of padded copies (odd widths, 1.25 2^30 multiply-adds) in 25 slices, in two and in one; a little less work, without copies.
 @pytest.mark.parametrize("dtype", HALVES, ids=NAMES)
 @pytest.mark.parametrize("tokens,k,experts,K,N", [(1500, 2, 9, 1032, 1288), (33800, 2, 130, 72, 40), (1500, 2, 9, 520, 776),
-                                                  (4400, 2, 8, 264, 520), (40400, 2, 5, 203, 131)])
+                                                  (4400, 2, 8, 264, 520), (40400, 2, 5, 203, 131), (2000, 2, 4, 515, 1027),
+                                                  (900, 2, 5, 1003, 777), (800, 2, 5, 1003, 777)])
 @pytest.mark.parametrize("f32_out", [True, False])
 def test_weight_gradient_in_16_bits(gpu, dtype, tokens, k, experts, K, N, f32_out):
     c = Case(gpu, dtype, tokens, k, experts, K, N)
