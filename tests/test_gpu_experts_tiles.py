@@ -233,3 +233,29 @@ def test_f32_matrices_of_more_than_2_21_a_side(gpu, ordered):
         assert torch.equal(dx[s:t], (a[s:t].double() @ wt[e].double().T.contiguous()).float())
         assert torch.equal(dw[e], (pick[s:t].double().T.contiguous() @ d[s:t].double()).float())
     assert bool((c[rows - 1] == 7).all()) and bool((dx[rows - 1] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", T.TYPES, ids=NAMES)
+@pytest.mark.parametrize("tokens,k,experts,K,N", [(4, 2, 3, 2100, 70), (40, 2, 8, 100, 72), (130, 2, 3, 136, 264), (130, 2, 3, 133, 131),
+                                                  (1500, 2, 4, 75, 501), (1500, 2, 4, 200, 1032)])
+def test_infinities_and_nan_stay_in_their_rows(gpu, dtype, tokens, k, experts, K, N):
+    """An infinity or NaN in a row of A or a matrix: what 64 bits give, and the other rows and experts as without it."""
+    c = Case(gpu, dtype, tokens, k, experts, K, N)
+    c.x[0, 3], c.x[tokens // 2, K - 1], c.x[tokens - 1, 0] = float("inf"), float("nan"), -float("inf")
+    c.rows = c.x[c.token]
+    c.w[0, 5, 1] = float("inf")
+    dz = c.normal(c.n, N)
+    y, dw = c.seven(c.n, N), c.seven(experts, K, N)
+    c.gemm(G.NN, c.held(c.x), c.held(c.w), c.held(y), c.d_off, c.d_order)
+    c.gemm(G.TN, c.held(c.x), c.held(dz), c.held(dw), c.d_off, c.d_order)
+    for e, a, b in c.each():
+        rows, w, d = c.rows[a:b].double(), c.w[e].double(), dz[a:b].double()
+        for got, m, o, adds in ((y[a:b], rows, w, K), (dw[e], rows.T.contiguous(), d, b - a + 32)):
+            if 0 in got.shape:
+                continue
+            want = m @ o
+            on = want.isfinite()
+            assert torch.equal(torch.where(on, 0.0, got.double()).nan_to_num(7.0, 8.0, 9.0),
+                               torch.where(on, 0.0, want).nan_to_num(7.0, 8.0, 9.0))
+            near(torch.where(on, got, 0.0), torch.where(on, want, 0.0),
+                 torch.where(on, m.abs().nan_to_num(0, 0, 0) @ o.abs().nan_to_num(0, 0, 0), 0.0), adds, G.F32)
