@@ -433,7 +433,7 @@ int rt_accuracy(rt_ctx* ctx, const rt_buf* logits, const rt_buf* labels, float* 
  * Operators of layers that learn from tokens; none has a counterpart in the
  * reference.  All enqueue only.  Float tensors are f32, bf16 or f16 where no
  * type is named; sums are f32, and a bf16 or f16 result is rounded once.  Outputs
- * share no memory with inputs or each other, but for rt_dropout's. */
+ * share no memory with inputs or each other, but where it is said. */
 
 /* y[i] = x[i] / (1 - q) where element i is kept, 0 where it is dropped (an
  * infinity or NaN too); q is p as the nearest whole number of 65536ths, p in
@@ -478,7 +478,8 @@ typedef enum { RT_SCORE_SOFTMAX = 0, RT_SCORE_SIGMOID = 1 } rt_score;
 int rt_route(rt_ctx* ctx, const rt_buf* logits, const rt_buf* bias, int score, size_t groups, size_t kept,
              int renormalise, float scale, rt_buf* ids, rt_buf* weights);
 /* The gradient of the logits (their type and shape) from the weights'; the
- * choice, and the bias, have none.  Ids >= experts take no part. */
+ * choice, and the bias, have none.  Ids >= experts take no part; an expert that is
+ * named twice counts twice.  dlogits may be the logits' own buffer. */
 int rt_route_backward(rt_ctx* ctx, const rt_buf* logits, int score, int renormalise, float scale, const rt_buf* ids,
                       const rt_buf* dweights, rt_buf* dlogits);
 

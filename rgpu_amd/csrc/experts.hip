@@ -791,10 +791,12 @@ hipError_t experts_launch(hipStream_t s, const ExpertArgs& args, float* rows) {
     };
     if (dma_ok<LAYOUT>(p)) {
       // 256x256 tiles read least, and have a CU to themselves: where they fill
-      // the chip, TN once (32 experts 2048 x 2048 over 32768 rows 387 us, 496 in
-      // 128x128 tiles; 64 of 512 x 512 over 8192 26.8 and 30.5; 8 of 1024 x 1024,
-      // 128 tiles, 36.5 and 28.7), the others twice and with rows for most of a tile (the
-      // 32 experts NN 329 and 382; 16 over 8192, 320 tiles, 120 and 108).
+      // the chip, TN once (32 experts 2048 x 2048 over 32768 rows 387 us, 501 in
+      // 128x128 tiles; 16 over 8192 140 and 182; 64 of 512 x 512 over 8192 27.4 and
+      // 30.4; 8 of 1024 x 1024, 128 tiles, 36.5 and 28.7), the others twice and with
+      // rows for most of a tile (the 32 experts NN 347 and 392, NT 324 and 362; 16 over
+      // 8192, 320 tiles, 120 and 108).  Experts drawn with probabilities e^(g / 2), g
+      // normal.
       if (LAYOUT == RT_TN ? tiles(256) >= 256 : tiles(256) >= 512 && mean >= 256)
         return experts_dma<DT, LAYOUT, 256, 256, 2, 4, 2>(s, p);
       // Where a 128x128 tile has a CU to itself, four stages (8 experts 1024 x

@@ -167,3 +167,18 @@ def test_weights_of_scores_whose_reciprocal_is_infinite(gpu, score, experts, k):
     want = np.zeros((5, experts))
     np.put_along_axis(want, got, w * (g - (w / 2.5 * g).sum(axis=1, keepdims=True)), axis=1)
     assert np.all(abs(gpu.download(dx) - want) <= 2.0 ** -22 * 2.5 * abs(g).max())
+
+
+@pytest.mark.parametrize("dtype", T.TYPES, ids=T.NAMES.get)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalise", [True, False])
+@pytest.mark.parametrize("tokens,experts,k", [(1, 8, 2), (37, 64, 4), (1000, 256, 8), (9, 1000, 30)])
+def test_route_backward_in_place(gpu, dtype, score, renormalise, tokens, experts, k):
+    rng = np.random.default_rng(tokens)
+    x, v = T.put(gpu, rng.normal(size=(tokens, experts)), dtype)
+    ids = T.words(gpu, T.route(v, k, score)[0])
+    g, dx = gpu.upload(rng.normal(size=(tokens, k)).astype(np.float32)), gpu.empty((tokens, experts), dtype)
+    gpu.route_backward(x, ids, g, dx, score=score, renormalise=renormalise)
+    want = gpu.download_f32(dx)
+    gpu.route_backward(x, ids, g, x, score=score, renormalise=renormalise)
+    assert np.array_equal(gpu.download_f32(x), want)
